@@ -114,6 +114,76 @@ int seraph_cross_entropy_grad(const float* logits, const uint32_t* targets, floa
  * been scheduled: tests use it to run that path.  A negative value changes nothing.  No reference counterpart. */
 void seraph_cross_entropy_exchange_spins(int spins);
 
+/* ---------------------------------------------------------------- objectives beside the cross entropy
+ * What a training step puts in the place of seraph_cross_entropy_grad when it does not learn the next token of a text:
+ * policy optimisation on sampled answers, preference pairs, distillation.  The reference trains with the cross entropy
+ * alone, so these have no counterpart there; they keep its conventions: FP32 logits [rows, cols], the loss per row
+ * undivided and the gradient divided by valid_rows (0 -> all gradients 0), grad may alias logits.
+ *
+ * A row is supervised when its target is below cols, its weight (where the op has weights) is not 0 and, with
+ * seq_starts, it lies in a sequence and is not that sequence's last token.  Any other row is not read: its gradient
+ * row and its per-row results are zeros.  Rows behind the last sequence count among those.  Within a supervised row
+ * a logit of -inf is an entry that cannot be chosen (probability and gradient 0).
+ * Any cols and any 4-byte aligned buffers are taken.  Results do not depend on the order in which workgroups run.
+ * A call without rows or columns does nothing.  ws needs 16-byte alignment; two calls that may overlap need scratch of
+ * their own.  No call allocates, waits or clears by memset, so all of them can be captured into a graph. */
+
+/* logp[r] = log softmax(logits[r])[targets[r]]; optional (NULL: not wanted) lse[r] = logsumexp of the row and
+ * entropy[r] = -sum p log p.  Forward only, for scoring and for the reference / sampling policy's pass. */
+size_t seraph_token_logprobs_ws_bytes(int64_t rows, int64_t cols);
+int seraph_token_logprobs(const float* logits, const uint32_t* targets, float* logp, float* lse, float* entropy,
+                          const uint32_t* seq_starts, int batch, int64_t rows, int64_t cols,
+                          void* ws, size_t ws_bytes, seraph_stream_t s);
+
+/* Clipped policy loss.  With logp as above and rho = exp(logp - old_logp):
+ *   loss_rows[r] = w (-min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef k - entropy_coef H),
+ *   k = exp(ref_logp - logp) - (ref_logp - logp) - 1   (the non-negative one-sample estimate of KL(policy || reference)),
+ * H the entropy of the row, A = advantages[r], w = weights[r] (NULL: 1); grad = d(sum of loss_rows)/d logits / valid_rows.
+ * ref_logp is needed where kl_coef != 0 or kl_rows is wanted.  logp_rows, kl_rows, entropy_rows: optional, unweighted. */
+typedef struct { float clip_low, clip_high, kl_coef, entropy_coef; } seraph_policy_options_t;
+size_t seraph_policy_grad_ws_bytes(int64_t rows, int64_t cols);
+int seraph_policy_grad(const float* logits, const uint32_t* actions, const float* advantages, const float* old_logp,
+                       const float* ref_logp, const float* weights, float* grad, float* loss_rows,
+                       float* logp_rows, float* kl_rows, float* entropy_rows, const seraph_policy_options_t* options,
+                       const uint32_t* seq_starts, int batch, int64_t rows, int64_t cols, int64_t valid_rows,
+                       void* ws, size_t ws_bytes, seraph_stream_t s);
+
+/* Preference loss over pairs: sequences 2i (chosen) and 2i + 1 (rejected) of seq_starts (2 pairs + 1 offsets).
+ *   score of a sequence = sum over its supervised rows of (logp - ref_logp)   (ref_logp NULL: 0),
+ * divided by their number when average != 0; gap = score(chosen) - score(rejected), h = beta gap - margin:
+ *   SIGMOID  -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h)
+ *   HINGE    max(0, 1 - h)
+ *   SQUARED  (gap - 1 / (2 beta))^2
+ * loss_pairs[pairs], scores[2 pairs] (optional), logp_rows[rows] (optional); grad = d(mean of loss_pairs)/d logits.
+ * A sequence without a supervised row has the score 0 and no gradient. */
+#define SERAPH_PREFERENCE_SIGMOID 0
+#define SERAPH_PREFERENCE_HINGE   1
+#define SERAPH_PREFERENCE_SQUARED 2
+typedef struct { int kind; float beta, label_smoothing, margin; int average; } seraph_preference_options_t;
+size_t seraph_preference_grad_ws_bytes(int64_t rows, int64_t cols);
+int seraph_preference_grad(const float* logits, const uint32_t* targets, const float* ref_logp, float* grad,
+                           float* loss_pairs, float* scores, float* logp_rows, const seraph_preference_options_t* options,
+                           const uint32_t* seq_starts, int pairs, int64_t rows, int64_t cols,
+                           void* ws, size_t ws_bytes, seraph_stream_t s);
+
+/* Distillation from the top_k logits that a teacher listed for each row (teacher_ids [rows, top_k], ids >= cols are
+ * skipped, an id listed twice adds its parts; teacher_logits of the given type).  With T = temperature:
+ *   q = softmax of the listed logits / T, or exp(logit / T - teacher_lse[r]) where teacher_lse (the teacher's
+ *       logsumexp of all its logits / T) is given; what the list leaves out is then left out of the loss,
+ *   loss_rows[r] = w (soft_coef sum_k q_k (log q_k - log softmax(logits[r] / T)[id_k]) + hard_coef (-log softmax(logits[r])[targets[r]])),
+ * grad = d(sum of loss_rows)/d logits / valid_rows (soft_coef = T^2 keeps its size as T grows).  targets (optional, needed
+ * where hard_coef != 0) does not make a row unsupervised here: an id >= cols only has no hard part.  top_k is at most 1024. */
+#define SERAPH_TYPE_F32  0
+#define SERAPH_TYPE_F16  1
+#define SERAPH_TYPE_BF16 2
+typedef struct { float temperature, soft_coef, hard_coef; int teacher_type; } seraph_distill_options_t;
+size_t seraph_distill_grad_ws_bytes(int64_t rows, int64_t cols, int64_t top_k);
+int seraph_distill_grad(const float* logits, const uint32_t* teacher_ids, const void* teacher_logits, const float* teacher_lse,
+                        const uint32_t* targets, const float* weights, float* grad, float* loss_rows,
+                        const seraph_distill_options_t* options, const uint32_t* seq_starts, int batch,
+                        int64_t rows, int64_t cols, int64_t top_k, int64_t valid_rows,
+                        void* ws, size_t ws_bytes, seraph_stream_t s);
+
 /* ---------------------------------------------------------------- GEMM family */
 /* vulkan_matmul (include/vulkan_backend.h:431-433, shaders/matmul.comp) and
  * vulkan_matmul_transpose (include/vulkan_backend.h:439-442, shaders/matmul_transpose.comp:35-169):

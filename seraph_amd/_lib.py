@@ -27,11 +27,37 @@ def kernels():
                      "seraph_rmsnorm_backward_ws_bytes", "seraph_embedding_backward_ws_bytes",
                      "seraph_gemm_scaled_ws_bytes", "seraph_rmsnorm_backward_static_max_bytes"):
             getattr(lib, name).restype = C.c_size_t
+        _bind_objectives(lib)
         lib.seraph_gemm_grouped_kernel_name.restype = C.c_char_p
         lib.seraph_gemm_chain_kernel_name.restype = C.c_char_p
         lib.seraph_gemm_kernel_name.restype = C.c_char_p
         _kernels = lib
     return _kernels
+
+
+class PolicyOptions(C.Structure):
+    _fields_ = [("clip_low", C.c_float), ("clip_high", C.c_float), ("kl_coef", C.c_float), ("entropy_coef", C.c_float)]
+
+
+class PreferenceOptions(C.Structure):
+    _fields_ = [("kind", C.c_int), ("beta", C.c_float), ("label_smoothing", C.c_float), ("margin", C.c_float), ("average", C.c_int)]
+
+
+class DistillOptions(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("soft_coef", C.c_float), ("hard_coef", C.c_float), ("teacher_type", C.c_int)]
+
+
+def _bind_objectives(lib):
+    """Argument types of the objectives over logits: plain Python numbers and addresses then go in as they are."""
+    p, i, n, z = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
+    for name, args in (("seraph_token_logprobs", [n, n]), ("seraph_policy_grad", [n, n]), ("seraph_preference_grad", [n, n]),
+                       ("seraph_distill_grad", [n, n, n])):
+        query = getattr(lib, name + "_ws_bytes")
+        query.restype, query.argtypes = z, args
+    lib.seraph_token_logprobs.argtypes = [p] * 6 + [i, n, n, p, z, p]
+    lib.seraph_policy_grad.argtypes = [p] * 11 + [C.POINTER(PolicyOptions), p, i, n, n, n, p, z, p]
+    lib.seraph_preference_grad.argtypes = [p] * 7 + [C.POINTER(PreferenceOptions), p, i, n, n, p, z, p]
+    lib.seraph_distill_grad.argtypes = [p] * 8 + [C.POINTER(DistillOptions), p, i, n, n, n, n, p, z, p]
 
 
 def backend():

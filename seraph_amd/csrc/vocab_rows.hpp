@@ -1,0 +1,115 @@
+// vocab_rows.hpp - what the objectives over vocabulary logits share: which rows are supervised, how a row is
+// addressed, reductions over a workgroup, and the exponentials.
+//
+// All of them are a softmax over rows of `cols` logits and, for the gradient, one value per logit that follows from
+// the logit and a few numbers of its row.  At six to ten operations per eight bytes every kernel here is bound by
+// memory; what differs between them is how often a logit crosses it.
+#pragma once
+
+#include <math.h>
+
+#include "common.hpp"
+
+namespace seraph {
+
+constexpr float kLowest = -3.402823466e38f;       // the type's lowest value: a maximum over nothing, or over masked logits
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4a4 __attribute__((ext_vector_type(4), aligned(4)));      // 16 bytes on a 4-byte boundary
+
+// What a row needs besides its maximum m and its sum of exp((z - m) / T):
+enum Extra {
+    kNone,        // nothing
+    kEntropy,     // the sum of exp(z - m) (z - m)      (T = 1)
+    kSecond       // the sum of exp(z - m), beside the one at T
+};
+
+struct RowStats { float m, s, x; };
+
+// The factor log2(e) / T in two parts.  Its FP32 rounding alone (1.3e-8 of it at T = 1) shifts every argument the same way,
+// which the logarithm of a sum keeps: over the hundreds of tokens of a sequence's score that is an error of 1e-5, where
+// the second part leaves 1e-7.
+struct ExpScale {
+    float hi, lo;
+    static ExpScale of(double inv_temp) {
+        const double k = 1.4426950408889634074 * inv_temp;
+        float hi = (float)k;
+        if ((double)hi >= k) hi = nextafterf(hi, 0.0f);           // both parts positive: -inf times them adds up to -inf
+        return ExpScale{hi, (float)(k - (double)hi)};
+    }
+};
+constexpr ExpScale kUnitScale{1.442695021629333f, 1.92596298909109e-8f};      // ExpScale::of(1)
+
+// exp((z - m) / T).  The difference is formed first: m k could overflow where every logit of a row is the type's
+// lowest value, and (z - m) k keeps the bits that fma(z, k, -m k) would lose for a large m.
+__device__ __forceinline__ float exp_of(float z, float m, ExpScale k) {
+    const float d = z - m;
+    return __builtin_amdgcn_exp2f(fmaf(d, k.hi, d * k.lo));
+}
+
+template <int EXTRA>
+__device__ __forceinline__ float extra_of(float z, float m, float e) {
+    if (EXTRA == kEntropy) return e > 0.0f ? e * (z - m) : (e == 0.0f ? 0.0f : e);      // exp(-inf) (-inf) counts 0, NaN stays
+    if (EXTRA == kSecond) return exp_of(z, m, kUnitScale);
+    return 0.0f;
+}
+
+template <int BLOCK>
+__device__ __forceinline__ float block_max(float v, float* lds) {
+    v = wave_max(v);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = lds[0];
+#pragma unroll
+    for (int w = 1; w < BLOCK / 64; w++) r = fmaxf(r, lds[w]);
+    return r;
+}
+template <int BLOCK, class T>
+__device__ __forceinline__ T block_sum(T v, T* lds) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    T r = lds[0];
+#pragma unroll
+    for (int w = 1; w < BLOCK / 64; w++) r += lds[w];
+    return r;
+}
+
+// A row of floats that need not start on a 16-byte boundary nor hold a multiple of four: `head` single values up to the
+// first boundary, n4 vectors, `tail` single values.  Lanes 0..3 of one workgroup hold the head, lanes 4..7 the tail.
+struct RowShape {
+    int head, n4, tail;
+    __device__ __forceinline__ RowShape(const float* row, int64_t cols) {
+        const int to_boundary = (int)((4u - ((unsigned)(reinterpret_cast<uintptr_t>(row) >> 2) & 3u)) & 3u);
+        head = to_boundary < cols ? to_boundary : (int)cols;
+        n4 = (int)((cols - head) >> 2);
+        tail = (int)((cols - head) & 3);
+    }
+    // the column of this lane's single value, -1 where it has none
+    __device__ __forceinline__ int64_t single(int lane) const {
+        if (lane < head) return lane;
+        if (lane >= 4 && lane < 4 + tail) return (int64_t)head + (int64_t)n4 * 4 + (lane - 4);
+        return -1;
+    }
+};
+
+// Which rows are supervised.
+struct Supervision {
+    const uint32_t* targets;       // NULL: the op has rows without targets
+    const float* weights;          // NULL: all 1
+    const uint32_t* seq_starts;    // NULL: one sequence, whose last row counts like the others
+    int batch;
+    int64_t cols;
+    __device__ __forceinline__ bool in_sequence(int64_t row) const {
+        if (!seq_starts) return true;
+        const int sq = find_seq(seq_starts, batch, row);
+        return sq < batch && row + 1 < (int64_t)seq_starts[sq + 1];
+    }
+    __device__ __forceinline__ bool live(int64_t row) const {
+        if (targets && (int64_t)targets[row] >= cols) return false;
+        if (weights && weights[row] == 0.0f) return false;
+        return in_sequence(row);
+    }
+};
+
+}  // namespace seraph

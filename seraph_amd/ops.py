@@ -9,7 +9,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import check, kernels
+from ._lib import DistillOptions, PolicyOptions, PreferenceOptions, SeraphError, check, kernels
 
 i64, f32, sz = C.c_int64, C.c_float, C.c_size_t
 
@@ -81,6 +81,169 @@ def cross_entropy_grad(logits, targets, valid_rows, seq_starts=None, grad=None):
     check(kernels().seraph_cross_entropy_grad(_p(logits), _p(targets), _p(grad), _p(loss), _p(seq_starts),
                                               C.c_int(_batch(seq_starts)), i64(rows), i64(cols), i64(valid_rows),
                                               _stream()), "cross_entropy_grad")
+    return grad, loss
+
+
+# ---------------------------------------------------------------- objectives beside the cross entropy
+PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "squared": 2}
+TEACHER_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _expect(op, name, t, dtypes, shape, device):
+    """The address of an argument after its type, shape, layout and device have been checked; None for None."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise SeraphError(f"{op}: {name} has to be contiguous {'/'.join(str(d) for d in dtypes)} {shape} on {device}; got {got}")
+    return t.data_ptr()
+
+
+_F32 = (torch.float32,)
+_IDS = (torch.int32, torch.uint32)
+
+
+def _logits(op, logits):
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda or not logits.is_contiguous():
+        raise SeraphError(f"{op}: logits have to be a contiguous float32 CUDA tensor [rows, cols]")
+    if logits.shape[1] == 0:
+        raise SeraphError(f"{op}: logits without columns")
+    return logits.shape[0], logits.shape[1], logits.device
+
+
+def _starts(op, seq_starts, device):
+    if seq_starts is None:
+        return None, 1
+    if not isinstance(seq_starts, torch.Tensor) or seq_starts.dim() != 1 or seq_starts.numel() < 2:
+        raise SeraphError(f"{op}: seq_starts has to be a tensor of at least two offsets")
+    return _expect(op, "seq_starts", seq_starts, _IDS, tuple(seq_starts.shape), device), seq_starts.numel() - 1
+
+
+def _scratch(nbytes, device):
+    """Scratch of the call's own: what the caching allocator hands out is ordered by the stream (and by the graph that
+    is being captured), so two streams or two captured graphs never share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class _on:
+    """Makes `device` the current one for a call, where it is not."""
+
+    def __init__(self, device):
+        self.device, self.before = device.index, None
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        if now != self.device:
+            self.before = now
+            torch.cuda.set_device(self.device)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
+
+
+def token_logprobs(logits, targets, seq_starts=None, want_lse=False, want_entropy=False):
+    """(log-probability of each row's target, the row's logsumexp or None, its entropy or None); zeros where a row is not
+    supervised (a target outside [0, cols), the last token of a packed sequence)."""
+    op = "token_logprobs"
+    rows, cols, device = _logits(op, logits)
+    t, (st, batch) = _expect(op, "targets", targets, _IDS, (rows,), device), _starts(op, seq_starts, device)
+    logp = torch.empty(rows, dtype=torch.float32, device=device)
+    lse = torch.empty_like(logp) if want_lse else None
+    entropy = torch.empty_like(logp) if want_entropy else None
+    k = kernels()
+    nbytes = k.seraph_token_logprobs_ws_bytes(rows, cols)
+    ws = _scratch(nbytes, device)
+    with _on(device) as stream:
+        check(k.seraph_token_logprobs(logits.data_ptr(), t, logp.data_ptr(), _ptr(lse), _ptr(entropy), st, batch, rows, cols,
+                                      _ptr(ws), nbytes, stream), op)
+    return logp, lse, entropy
+
+
+def policy_grad(logits, actions, advantages, old_logp, valid_rows, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_coef=0.0,
+                entropy_coef=0.0, seq_starts=None, grad=None, want_entropy=False):
+    """Clipped policy loss with an optional KL term and entropy bonus: (gradient with respect to the logits, loss of each
+    row, its log-probability, its KL estimate or None without ref_logp, its entropy or None unless it is in the loss or
+    wanted).  grad may be the logits themselves."""
+    op = "policy_grad"
+    rows, cols, device = _logits(op, logits)
+    a = _expect(op, "actions", actions, _IDS, (rows,), device)
+    adv, old, ref, w = (_expect(op, n, v, _F32, (rows,), device) for n, v in
+                        (("advantages", advantages), ("old_logp", old_logp), ("ref_logp", ref_logp), ("weights", weights)))
+    st, batch = _starts(op, seq_starts, device)
+    grad = torch.empty_like(logits) if grad is None else grad
+    g = _expect(op, "grad", grad, _F32, (rows, cols), device)
+    loss = torch.empty(rows, dtype=torch.float32, device=device)
+    logp = torch.empty_like(loss)
+    kl = torch.empty_like(loss) if ref_logp is not None else None
+    entropy = torch.empty_like(loss) if want_entropy or entropy_coef else None
+    k = kernels()
+    nbytes = k.seraph_policy_grad_ws_bytes(rows, cols)
+    ws = _scratch(nbytes, device)
+    options = PolicyOptions(clip[0], clip[1], kl_coef, entropy_coef)
+    with _on(device) as stream:
+        check(k.seraph_policy_grad(logits.data_ptr(), a, adv, old, ref, w, g, loss.data_ptr(), logp.data_ptr(), _ptr(kl), _ptr(entropy),
+                                   options, st, batch, rows, cols, valid_rows, _ptr(ws), nbytes, stream), op)
+    return grad, loss, logp, kl, entropy
+
+
+def preference_grad(logits, targets, seq_starts, ref_logp=None, kind="sigmoid", beta=0.1, label_smoothing=0.0, margin=0.0,
+                    average=False, grad=None):
+    """Preference loss over the pairs (2i chosen, 2i + 1 rejected) of the packed sequences: (gradient of the mean loss with
+    respect to the logits, loss of each pair, score of each sequence).  grad may be the logits themselves."""
+    op = "preference_grad"
+    rows, cols, device = _logits(op, logits)
+    t, ref = _expect(op, "targets", targets, _IDS, (rows,), device), _expect(op, "ref_logp", ref_logp, _F32, (rows,), device)
+    st, batch = _starts(op, seq_starts, device)
+    if st is None or batch % 2:
+        raise SeraphError(f"{op}: seq_starts has to hold the offsets of an even number of sequences")
+    if rows == 0:
+        raise SeraphError(f"{op}: logits without rows")
+    if kind not in PREFERENCE_KINDS:
+        raise SeraphError(f"{op}: kind has to be one of {sorted(PREFERENCE_KINDS)}; got {kind!r}")
+    grad = torch.empty_like(logits) if grad is None else grad
+    g = _expect(op, "grad", grad, _F32, (rows, cols), device)
+    loss = torch.empty(batch // 2, dtype=torch.float32, device=device)
+    scores = torch.empty(batch, dtype=torch.float32, device=device)
+    k = kernels()
+    nbytes = k.seraph_preference_grad_ws_bytes(rows, cols)
+    ws = _scratch(nbytes, device)
+    options = PreferenceOptions(PREFERENCE_KINDS[kind], beta, label_smoothing, margin, 1 if average else 0)
+    with _on(device) as stream:
+        check(k.seraph_preference_grad(logits.data_ptr(), t, ref, g, loss.data_ptr(), scores.data_ptr(), None, options, st, batch // 2,
+                                       rows, cols, _ptr(ws), nbytes, stream), op)
+    return grad, loss, scores
+
+
+def distill_grad(logits, teacher_ids, teacher_logits, valid_rows, temperature=1.0, soft_coef=1.0, hard_coef=0.0, targets=None,
+                 teacher_lse=None, weights=None, seq_starts=None, grad=None):
+    """Distillation from the logits [rows, top_k] that a teacher listed (float32, float16 or bfloat16; ids outside [0, cols)
+    are skipped): (gradient with respect to the logits, loss of each row).  grad may be the logits themselves."""
+    op = "distill_grad"
+    rows, cols, device = _logits(op, logits)
+    if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dim() != 2:
+        raise SeraphError(f"{op}: teacher_ids have to be a tensor [rows, top_k]")
+    top_k = teacher_ids.shape[1]
+    ids = _expect(op, "teacher_ids", teacher_ids, _IDS, (rows, top_k), device)
+    tl = _expect(op, "teacher_logits", teacher_logits, tuple(TEACHER_TYPES), (rows, top_k), device)
+    t = _expect(op, "targets", targets, _IDS, (rows,), device)
+    w, tlse = _expect(op, "weights", weights, _F32, (rows,), device), _expect(op, "teacher_lse", teacher_lse, _F32, (rows,), device)
+    st, batch = _starts(op, seq_starts, device)
+    grad = torch.empty_like(logits) if grad is None else grad
+    g = _expect(op, "grad", grad, _F32, (rows, cols), device)
+    loss = torch.empty(rows, dtype=torch.float32, device=device)
+    k = kernels()
+    nbytes = k.seraph_distill_grad_ws_bytes(rows, cols, top_k)
+    ws = _scratch(nbytes, device)
+    options = DistillOptions(temperature, soft_coef, hard_coef, TEACHER_TYPES[teacher_logits.dtype])
+    with _on(device) as stream:
+        check(k.seraph_distill_grad(logits.data_ptr(), ids, tl, tlse, t, w, g, loss.data_ptr(), options, st, batch, rows, cols, top_k,
+                                    valid_rows, _ptr(ws), nbytes, stream), op)
     return grad, loss
 
 

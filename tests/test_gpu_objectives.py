@@ -1,0 +1,453 @@
+"""The objectives over logits (seraph_token_logprobs, _policy_grad, _preference_grad, _distill_grad) against their
+64-bit definitions, within tolerances that tests/objectives_ref.py derives from the arithmetic."""
+import numpy as np
+import pytest
+import torch
+
+from tests import objectives_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+# one column; fewer columns than a vector; widths around each kernel's limits, multiples of four and not; beyond the
+# longest row that fits registers
+COLS = [1, 2, 3, 5, 63, 64, 257, 1000, 1023, 1024, 1029, 2048, 4099, 8192, 16385, 32768, 32769, 33001, 50021, 65536, 151936, 151935]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from seraph_amd import ops as o
+    o.init(0)
+    return o
+
+
+def dev(a, shift=0):
+    """On the device; with a shift, at an address that is 4 shift bytes past a 16-byte boundary."""
+    if a is None:
+        return None
+    a = np.ascontiguousarray(a)
+    if a.dtype == np.uint32:
+        a = a.view(np.int32)
+    t = torch.from_numpy(a)
+    if not shift:
+        return t.cuda()
+    room = torch.empty(t.numel() + shift, dtype=t.dtype, device="cuda")
+    view = room[shift:].view(t.shape)
+    view.copy_(t)
+    return view
+
+
+def check(what, got, want, tol):
+    got = got.detach().cpu().numpy().astype(np.float64)
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid="ignore"):
+        bad = ~(same | (np.abs(got - want) <= tol))
+    if bad.any():
+        i = np.unravel_index(np.argmax(np.where(bad, np.abs(got - want) / tol, 0)), bad.shape)
+        raise AssertionError(f"{what}: {bad.sum()} of {bad.size} off; worst at {i}: got {got[i]:.9g} want {want[i]:.9g} tolerance {tol[i]:.3g}")
+
+
+def make(rows, cols, seed, spread=2.0):
+    r = np.random.default_rng(seed)
+    z = (spread * r.standard_normal((rows, cols))).astype(np.float32)
+    t = r.integers(0, cols, rows).astype(np.uint32)
+    return r, z, t
+
+
+def target_logp(z, t):
+    out = np.zeros(len(z))
+    for i in range(len(z)):
+        if t[i] < z.shape[1]:
+            out[i] = ref.log_softmax(z[i:i + 1].astype(np.float64))[0, t[i]]
+    return out
+
+
+def policy_inputs(r, z, t):
+    """old policies on both sides of both bounds and well away from them, whatever the logits"""
+    logp = target_logp(z, t)
+    steps = np.array([0.05, -0.07, 0.6, -0.6, 0.1, -0.45])
+    old = (logp - steps[np.arange(len(z)) % 6]).astype(np.float32)
+    refl = (logp + 0.3 * r.standard_normal(len(z))).astype(np.float32)
+    adv = np.where(np.arange(len(z)) // 6 % 2 == 0, 1.0, -1.0) * (0.5 + r.random(len(z)))
+    return adv.astype(np.float32), old, refl
+
+
+def run_policy(ops, z, t, adv, old, valid, refl=None, weights=None, starts=None, kl=0.0, ent=0.0, shift=0, gshift=None, in_place=False):
+    Z = dev(z, shift)
+    grad = Z if in_place else None
+    if gshift is not None:
+        grad = dev(np.full(z.shape, np.nan, np.float32), gshift)
+    got = ops.policy_grad(Z, dev(t), dev(adv), dev(old), valid, ref_logp=dev(refl), weights=dev(weights), clip=(0.2, 0.3), kl_coef=kl,
+                          entropy_coef=ent, seq_starts=dev(starts), grad=grad, want_entropy=bool(ent))
+    torch.cuda.synchronize()
+    return dict(zip(("grad", "loss", "logp", "kl", "entropy"), got))
+
+
+def compare(got, pair, what):
+    want, tol = pair
+    for k, v in got.items():
+        if v is not None:
+            check(f"{what} {k}", v, want[k], tol[k])
+
+
+@pytest.mark.parametrize("cols", COLS)
+def test_token_logprobs(ops, cols):
+    rows = 5
+    r, z, t = make(rows, cols, cols)
+    t[1] = cols                                                   # not supervised
+    for entropy in (False, True):
+        logp, lse, ent = ops.token_logprobs(dev(z), dev(t), want_lse=True, want_entropy=entropy)
+        compare(dict(logp=logp, lse=lse, entropy=ent), ref.token_logprobs(z, t), f"{cols}")
+    one, none, _ = ops.token_logprobs(dev(z), dev(t))
+    assert none is None and torch.equal(one, ops.token_logprobs(dev(z), dev(t), want_lse=True)[0])
+
+
+@pytest.mark.parametrize("cols", COLS)
+def test_policy(ops, cols):
+    rows = 13
+    r, z, t = make(rows, cols, cols + 1)
+    t[3] = 0xffffffff
+    adv, old, refl = policy_inputs(r, z, t)
+    w = (0.5 + r.random(rows)).astype(np.float32)
+    w[4] = 0
+    for kw in (dict(), dict(refl=refl, kl=0.05, weights=w), dict(refl=refl, kl=0.05, ent=0.01, weights=w)):
+        got = run_policy(ops, z, t, adv, old, rows - 2, **kw)
+        want = ref.policy(z, t, adv, old, rows - 2, ref=kw.get("refl"), weights=kw.get("weights"), clip=(0.2, 0.3), kl_coef=kw.get("kl", 0.0),
+                          entropy_coef=kw.get("ent", 0.0))
+        compare(got, want, f"{cols} {sorted(kw)}")
+        again = run_policy(ops, z, t, adv, old, rows - 2, **kw)
+        inside = run_policy(ops, z, t, adv, old, rows - 2, in_place=True, **kw)
+        for k in got:
+            assert got[k] is None or (torch.equal(got[k], again[k]) and torch.equal(got[k], inside[k])), (cols, k)
+    zero = run_policy(ops, z, t, adv, old, 0)
+    assert (zero["grad"] == 0).all()
+
+
+@pytest.mark.parametrize("cols", COLS)
+@pytest.mark.parametrize("kind,average", [("sigmoid", False), ("hinge", True), ("squared", True)])
+def test_preference(ops, cols, kind, average):
+    starts = np.array([0, 3, 4, 9, 13, 13, 20], np.uint32)        # ragged; a pair with an empty sequence
+    rows = 22                                                     # two rows behind the last sequence
+    r, z, t = make(rows, cols, cols + 2)
+    t[[0, 5, 16]] = cols
+    refl = (target_logp(z, t) + 0.3 * r.standard_normal(rows)).astype(np.float32)
+    for kw in (dict(ref=refl), dict(ref=None)):
+        want = ref.preference(z, t, starts.astype(int), kind=kind, beta=0.3, eps=0.1, margin=0.2, average=average, **kw)
+        res = []
+        for in_place in (False, True, False):
+            Z = dev(z)
+            grad = Z if in_place else dev(np.full(z.shape, np.nan, np.float32))
+            g, loss, scores = ops.preference_grad(Z, dev(t), dev(starts), ref_logp=dev(kw["ref"]), kind=kind, beta=0.3, label_smoothing=0.1,
+                                                  margin=0.2, average=average, grad=grad)
+            res.append((g, loss, scores))
+        compare(dict(grad=res[0][0], loss=res[0][1], scores=res[0][2]), want, f"{cols} {kind}")
+        for other in res[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(res[0], other))
+
+
+TYPES = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.bfloat16}
+
+
+def distill_inputs(r, z, top_k, dtype):
+    rows, cols = z.shape
+    ids = np.stack([r.permutation(cols)[:top_k] if cols >= top_k else r.integers(0, cols, top_k) for _ in range(rows)]).astype(np.uint32)
+    teacher = torch.from_numpy((3 * r.standard_normal((rows, top_k))).astype(np.float32)).to(TYPES[dtype])
+    return ids, teacher
+
+
+def run_distill(ops, z, ids, teacher, valid, in_place=False, shift=0, **kw):
+    Z = dev(z, shift)
+    grad = Z if in_place else dev(np.full(z.shape, np.nan, np.float32), shift)
+    for k in ("targets", "teacher_lse", "weights", "seq_starts"):
+        if k in kw:
+            kw[k] = dev(kw[k])
+    g, loss = ops.distill_grad(Z, dev(ids), teacher.cuda(), valid, grad=grad, **kw)
+    return dict(grad=g, loss=loss)
+
+
+@pytest.mark.parametrize("cols", COLS)
+@pytest.mark.parametrize("top_k,dtype,temperature,hard", [(1, "float32", 1.0, 0.0), (7, "bfloat16", 2.0, 0.3), (64, "float16", 1.0, 0.3), (300, "float32", 0.5, 0.0)])
+def test_distill(ops, cols, top_k, dtype, temperature, hard):
+    rows = 6
+    r, z, t = make(rows, cols, cols + 3)
+    ids, teacher = distill_inputs(r, z, top_k, dtype)             # with few columns: every id many times
+    if cols > 8:
+        ids[0, 0] = t[0]                                          # the label among the listed
+    ids[1, top_k // 2:] = cols + 5                                # a shorter list
+    ids[2] = 0xffffffff                                           # no list at all
+    t[3] = cols
+    w = (0.5 + r.random(rows)).astype(np.float32)
+    w[4] = 0
+    kw = dict(temperature=temperature, weights=w, targets=t)
+    want = ref.distill(z, ids, teacher.float().numpy(), rows - 1, soft=0.7, hard=hard, **kw)
+    got = run_distill(ops, z, ids, teacher, rows - 1, soft_coef=0.7, hard_coef=hard, **kw)
+    compare(got, want, f"{cols} {top_k}")
+    again = run_distill(ops, z, ids, teacher, rows - 1, soft_coef=0.7, hard_coef=hard, **kw)
+    inside = run_distill(ops, z, ids, teacher, rows - 1, soft_coef=0.7, hard_coef=hard, in_place=True, **kw)
+    for k in got:
+        assert torch.equal(got[k], again[k]) and torch.equal(got[k], inside[k]), k
+
+
+@pytest.mark.parametrize("cols", [37, 8192, 40003])
+def test_distill_longest_list_and_the_teachers_own_norm(ops, cols):
+    rows, top_k = 4, 1024
+    r, z, t = make(rows, cols, cols + 4)
+    ids = r.integers(0, cols, (rows, top_k)).astype(np.uint32)    # many ids listed twice
+    teacher = torch.from_numpy((2 * r.standard_normal((rows, top_k))).astype(np.float32))
+    teacher[0, 5:9] = -float("inf")
+    teacher[1] = -float("inf")                                    # a list without mass
+    lse = (np.log(top_k) + 3 + r.random(rows)).astype(np.float32)
+    for kw in (dict(), dict(teacher_lse=lse)):
+        want = ref.distill(z, ids, teacher.numpy(), rows, lse=kw.get("teacher_lse"), temperature=1.5)
+        compare(run_distill(ops, z, ids, teacher, rows, temperature=1.5, **kw), want, f"{cols} {sorted(kw)}")
+
+
+@pytest.mark.parametrize("cols", [6, 8192, 8191, 33001, 40000, 1300003])
+@pytest.mark.parametrize("shift,gshift", [(1, 1), (2, 3), (3, 0), (0, 2)])
+def test_buffers_off_the_16_byte_boundary(ops, cols, shift, gshift):
+    rows = 3 if cols < 10 ** 6 else 2
+    r, z, t = make(rows, cols, cols + 5)
+    adv, old, refl = policy_inputs(r, z, t)
+    got = run_policy(ops, z, t, adv, old, rows, refl=refl, kl=0.1, ent=0.02, shift=shift, gshift=gshift)
+    compare(got, ref.policy(z, t, adv, old, rows, ref=refl, clip=(0.2, 0.3), kl_coef=0.1, entropy_coef=0.02), f"{cols}")
+    lp, lse, ent = ops.token_logprobs(dev(z, shift), dev(t), want_lse=True, want_entropy=True)
+    compare(dict(logp=lp, lse=lse, entropy=ent), ref.token_logprobs(z, t), f"{cols}")
+    ids, teacher = distill_inputs(r, z, 5, "float32")
+    compare(run_distill(ops, z, ids, teacher, rows, shift=shift), ref.distill(z, ids, teacher.numpy(), rows), f"{cols}")
+    starts = np.array([0, 1, rows], np.uint32)
+    g, loss, scores = ops.preference_grad(dev(z, shift), dev(t), dev(starts), grad=dev(np.full(z.shape, np.nan, np.float32), gshift))
+    compare(dict(grad=g, loss=loss, scores=scores), ref.preference(z, t, starts.astype(int)), f"{cols}")
+
+
+@pytest.mark.parametrize("cols", [50, 8192, 40001])
+def test_rows_that_are_not_supervised_are_not_read(ops, cols):
+    """Prompts, the last tokens of sequences, empty sequences and rows behind the last sequence, all full of NaN and infinities."""
+    starts = np.array([0, 0, 4, 5, 5, 11, 12], np.uint32)
+    rows = 15
+    r, z, t = make(rows, cols, cols + 6)
+    t[[5, 7]] = cols
+    live = ref.supervised(rows, cols, t, None, starts.astype(int))
+    assert 0 < live.sum() < rows
+    adv, old, refl = policy_inputs(r, z, t)
+    for a in (adv, old, refl):
+        a[~live] = np.nan
+    clean = z.copy()
+    z[~live] = np.array([np.nan, np.inf, -np.inf], np.float32)[np.arange(cols) % 3]
+    s = starts.astype(int)
+    got = run_policy(ops, z, t, adv, old, 4, refl=refl, kl=0.1, ent=0.01, starts=starts, gshift=0)
+    compare(got, ref.policy(clean, t, adv, old, 4, ref=refl, clip=(0.2, 0.3), kl_coef=0.1, entropy_coef=0.01, starts=s), "policy")
+    lp, lse, ent = ops.token_logprobs(dev(z), dev(t), seq_starts=dev(starts), want_lse=True, want_entropy=True)
+    compare(dict(logp=lp, lse=lse, entropy=ent), ref.token_logprobs(clean, t, s), "logprobs")
+    g, loss, scores = ops.preference_grad(dev(z), dev(t), dev(starts), ref_logp=dev(refl), grad=dev(np.full(z.shape, np.nan, np.float32)))
+    compare(dict(grad=g, loss=loss, scores=scores), ref.preference(clean, t, s, ref=refl), "preference")
+    ids, teacher = distill_inputs(r, clean, 4, "float32")
+    inside = ref.supervised(rows, cols, None, None, s)
+    z2 = clean.copy()
+    z2[~inside] = np.nan
+    teacher[~inside] = float("nan")
+    compare(run_distill(ops, z2, ids, teacher, 4, seq_starts=starts, hard_coef=0.5, targets=t),
+            ref.distill(clean, ids, teacher.numpy(), 4, hard=0.5, targets=t, starts=s), "distill")
+    none = np.full(rows, cols, np.uint32)                         # nothing supervised at all
+    got = run_policy(ops, z, none, adv, old, 4, refl=refl, kl=0.1, starts=starts, gshift=0)
+    assert all((got[k] == 0).all() for k in ("grad", "loss", "logp", "kl"))
+
+
+@pytest.mark.parametrize("cols", [9, 1000, 8192, 33000, 151936])
+def test_masked_logits_inside_a_row(ops, cols):
+    """Entries of -inf and of the type's lowest value, rows where a single entry is left, rows of nothing but lowest values,
+    and values far from zero."""
+    rows = 12
+    r, z, t = make(rows, cols, cols + 7)
+    low = np.finfo(np.float32).min
+    t[:] = r.integers(0, 4, rows)
+    z[0, 4:] = -np.inf
+    z[1, 4:] = low
+    z[2] = -np.inf; z[2, t[2]] = 3.0
+    z[3] = low; z[3, t[3]] = 1.0
+    z[4] = low                                                    # uniform
+    z[5] += 1e4
+    z[6] -= 1e4
+    z[7, ::2] = -np.inf; z[7, t[7]] = 0.5
+    z[8] = 0.0
+    z[9, cols // 2] = 300.0
+    z[10, :] = -np.inf; z[10, t[10]] = low
+    z[11, 4:] = -1e30
+    adv, old, refl = policy_inputs(r, z, t)
+    got = run_policy(ops, z, t, adv, old, rows, refl=refl, kl=0.1, ent=0.01)
+    compare(got, ref.policy(z, t, adv, old, rows, ref=refl, clip=(0.2, 0.3), kl_coef=0.1, entropy_coef=0.01), "policy")
+    lp, lse, ent = ops.token_logprobs(dev(z), dev(t), want_lse=True, want_entropy=True)
+    compare(dict(logp=lp, lse=lse, entropy=ent), ref.token_logprobs(z, t), "logprobs")
+    starts = np.array([0, 6, 12], np.uint32)
+    g, loss, scores = ops.preference_grad(dev(z), dev(t), dev(starts), ref_logp=dev(refl))
+    compare(dict(grad=g, loss=loss, scores=scores), ref.preference(z, t, starts.astype(int), ref=refl), "preference")
+    ids = np.tile(np.arange(4, dtype=np.uint32), (rows, 1))
+    teacher = torch.from_numpy(r.standard_normal((rows, 4)).astype(np.float32))
+    teacher[(2, 3, 7, 10), :] = -float("inf")                     # mass only where the student can follow
+    for i in (2, 3, 7, 10):
+        teacher[i, int(t[i])] = 1.0
+    for temperature, hard in ((1.0, 0.0), (2.0, 0.5)):
+        want = ref.distill(z, ids, teacher.numpy(), rows, temperature=temperature, hard=hard, targets=t)
+        compare(run_distill(ops, z, ids, teacher, rows, temperature=temperature, hard_coef=hard, targets=t), want, f"distill {temperature}")
+
+
+@pytest.mark.parametrize("cols", [100, 8192, 40000])
+def test_nan_and_inf_stay_in_their_row(ops, cols):
+    r, z, t = make(6, cols, cols + 8)
+    z[1, 3] = np.nan
+    z[3, 5] = np.inf
+    z[4] = -np.inf
+    adv, old, refl = policy_inputs(r, z, t)
+    old[:], refl[:] = -5.0, -5.0
+    got = run_policy(ops, z, t, adv, old, 6, refl=refl, kl=0.1, ent=0.01)
+    for i in range(6):
+        assert torch.isnan(got["grad"][i]).all().item() == (i in (1, 3, 4)) and torch.isnan(got["logp"][i]).item() == (i in (1, 3, 4)), i
+        assert torch.isfinite(got["grad"][i]).all().item() == (i not in (1, 3, 4))
+    ids, teacher = distill_inputs(r, z, 3, "float32")
+    teacher[0, 1] = float("nan")
+    got = run_distill(ops, z, ids, teacher, 6)
+    for i in range(6):
+        assert torch.isnan(got["grad"][i]).all().item() == (i in (0, 1, 3, 4)), i
+
+
+@pytest.mark.parametrize("rows,cols", [(3000, 1029), (1, 151936), (700, 33000), (300, 65537)])
+def test_many_rows_and_one(ops, rows, cols):
+    """More rows than workgroups that fit the chip, and a single one; checked on the device in 64 bits by torch."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    z = torch.empty(rows, cols, device="cuda").normal_(0, 2, generator=g)
+    t = torch.randint(0, cols, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    lsm = torch.log_softmax(z.double(), 1)
+    want = lsm.gather(1, t.long()[:, None])[:, 0]
+    u = float(ref.unit(z[:1].cpu().numpy())[0, 0]) * 2            # the rows are alike; twice one row's bound
+    logp, _, ent = ops.token_logprobs(z, t, want_entropy=True)
+    assert ((logp.double() - want).abs() <= u + ref.HALF_STEP * want.abs()).all()
+    old = (want - 0.1).float()
+    adv = torch.ones(rows, device="cuda")
+    grad, loss, lp, _, _ = ops.policy_grad(z, t, adv, old, rows, weights=torch.full((rows,), 2.0, device="cuda"))
+    rho = torch.exp(want - old.double())
+    p = lsm.exp()
+    hot = torch.zeros_like(p).scatter_(1, t.long()[:, None], 1.0)
+    f = (2.0 / rows) * rho[:, None]
+    assert ((grad.double() - f * (p - hot)).abs() <= 4 * u * f * (p + hot)).all()
+    assert torch.equal(lp, logp)
+    k = 5
+    ids = torch.stack([torch.randperm(cols, device="cuda", generator=g)[:k] for _ in range(rows)]).to(torch.int32)
+    tl = torch.empty(rows, k, device="cuda").normal_(generator=g)
+    q = torch.softmax(tl.double(), 1)
+    grad, loss = ops.distill_grad(z, ids, tl, rows)
+    want_g = p.scatter_add(1, ids.long(), -q) / rows
+    assert ((grad.double() - want_g).abs() <= 4 * u * (p + torch.zeros_like(p).scatter_(1, ids.long(), q)) / rows).all()
+    wl = (q * (q.log() - lsm.gather(1, ids.long()))).sum(1)
+    assert ((loss.double() - wl).abs() <= 4 * u * (1 + wl.abs() + q.log().abs().max())).all()
+
+
+@pytest.mark.parametrize("cols", [13, 8192, 40001])
+def test_gradients_against_differences(ops, cols):
+    """The gradient of each op against central differences of the op's own loss, at entries that carry it.  With a step
+    of h = 1/16 the difference is off by h^2 |f'''| / 6, |f'''| at most the row's factor times 8, plus the loss's own
+    error (the bound of the 64-bit definition) over h."""
+    rows, h = 4, 1.0 / 16
+    r, z, t = make(rows, cols, cols + 9, spread=0.5)
+    z[np.arange(rows), t] += np.log(cols)                         # probabilities that differences can see
+    adv, old, refl = policy_inputs(r, z, t)
+    old = (target_logp(z, t) - 0.05).astype(np.float32)           # inside the bounds for every step
+    starts = np.array([0, 2, 4], np.uint32)
+    ids, teacher = distill_inputs(r, z, 3, "float32")
+    ids[:, 0] = t
+
+    def policy(x):
+        return run_policy(ops, x, t, adv, old, 1, refl=refl, kl=0.1, ent=0.01)
+
+    def pref(x):
+        g, loss, _ = ops.preference_grad(dev(x), dev(t), dev(starts), ref_logp=dev(refl), beta=0.5)
+        return dict(grad=g, loss=loss)
+
+    def dist(x):
+        return run_distill(ops, x, ids, teacher, 1, temperature=1.5, hard_coef=0.4, targets=t)
+    lt = {policy: ref.policy(z, t, adv, old, 1, ref=refl, clip=(0.2, 0.3), kl_coef=0.1, entropy_coef=0.01)[1]["loss"].sum(),
+          pref: ref.preference(z, t, starts.astype(int), ref=refl, beta=0.5)[1]["loss"].sum(),
+          dist: ref.distill(z, ids, teacher.numpy(), 1, temperature=1.5, hard=0.4, targets=t)[1]["loss"].sum()}
+    for f in (policy, pref, dist):
+        grad = f(z)["grad"].cpu().numpy().astype(np.float64)
+        for row in range(rows):
+            for c in (int(t[row]), int(ids[row, 1]), (int(t[row]) + 1) % cols):
+                a, b = z.copy(), z.copy()
+                a[row, c] += h
+                b[row, c] -= h
+                step = float(a[row, c]) - float(b[row, c])
+                d = (f(a)["loss"].double().sum() - f(b)["loss"].double().sum()).item() / step
+                if f is pref:
+                    d /= 1                                        # one pair: the mean is the loss
+                assert abs(d - grad[row, c]) <= h * h * 8 * 2.0 / 6 + 2 * 2 * lt[f] / step, (f.__name__, row, c, d, grad[row, c])
+
+
+def test_captured_and_replayed(ops):
+    """Each op captured into a graph, replayed on new inputs with eager work in between, against the eager result."""
+    for rows, cols in ((7, 8191), (9, 40000)):
+        r, z, t = make(rows, cols, cols)
+        adv, old, refl = policy_inputs(r, z, t)
+        ids, teacher = distill_inputs(r, z, 8, "float32")
+        starts = np.array([0, 3, rows], np.uint32)
+        Z, T, A, O, R, I, L, S = (dev(a) for a in (z, t, adv, old, refl, ids, teacher.numpy(), starts))
+        calls = (lambda: ops.policy_grad(Z, T, A, O, rows, ref_logp=R, kl_coef=0.1, entropy_coef=0.01),
+                 lambda: ops.preference_grad(Z, T, S, ref_logp=R), lambda: ops.distill_grad(Z, I, L, rows, targets=T, hard_coef=0.5, temperature=2.0),
+                 lambda: ops.token_logprobs(Z, T, want_lse=True, want_entropy=True))
+        for call in calls:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                call()
+            torch.cuda.current_stream().wait_stream(side)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = call()
+            for k in range(4):
+                Z.copy_(dev((2 * np.random.default_rng(100 + k).standard_normal((rows, cols))).astype(np.float32)))
+                want = call()
+                torch.cuda.synchronize()
+                g.replay()
+                torch.cuda.synchronize()
+                for a, b in zip(out, want):
+                    assert a is None or torch.equal(a, b)
+
+
+def test_two_streams_at_once(ops):
+    """Calls on two streams over long rows, started together, give what each gives alone."""
+    rows, cols = 600, 40001
+    data = []
+    for seed in (1, 2):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        z = torch.empty(rows, cols, device="cuda").normal_(0, 2, generator=g)
+        t = torch.randint(0, cols, (rows,), device="cuda", generator=g, dtype=torch.int32)
+        lp, _, _ = ops.token_logprobs(z, t)
+        data.append((z, t, lp, torch.ones(rows, device="cuda")))
+    alone = [ops.policy_grad(z, t, a, lp, rows) for z, t, lp, a in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    got = []
+    for _ in range(3):
+        for s, (z, t, lp, a) in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(ops.policy_grad(z, t, a, lp, rows))
+    torch.cuda.synchronize()
+    for i, res in enumerate(got):
+        assert all(x is None or torch.equal(x, y) for x, y in zip(res, alone[i % 2]))
+
+
+def test_wrapper_refusals(ops):
+    from seraph_amd._lib import SeraphError
+    z, t, f = torch.zeros(4, 8, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(4, device="cuda")
+    s = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    for bad in (lambda: ops.token_logprobs(z.half(), t), lambda: ops.token_logprobs(z.t(), t), lambda: ops.token_logprobs(z, t.long()),
+                lambda: ops.token_logprobs(z, t[:3]), lambda: ops.token_logprobs(z, t.cpu()), lambda: ops.token_logprobs(z[:, :0], t),
+                lambda: ops.policy_grad(z, t, f, f[:3], 4), lambda: ops.policy_grad(z, t, f, f, 4, kl_coef=0.1),
+                lambda: ops.policy_grad(z, t, f, f, 4, grad=z[:2]), lambda: ops.policy_grad(z, t, f, f, 4, clip=(-1.0, 0.2)),
+                lambda: ops.preference_grad(z, t, s[:2]), lambda: ops.preference_grad(z, t, None), lambda: ops.preference_grad(z, t, s, kind="x"),
+                lambda: ops.preference_grad(z, t, s, beta=0.0), lambda: ops.distill_grad(z, t, f, 4),
+                lambda: ops.distill_grad(z, t[:, None], f[:, None].double(), 4), lambda: ops.distill_grad(z, t[:, None], f[:, None], 4, hard_coef=1.0),
+                lambda: ops.distill_grad(z, t[:, None], f[:, None], 4, temperature=0.0),
+                lambda: ops.distill_grad(z, torch.zeros(4, 1025, dtype=torch.int32, device="cuda"), torch.zeros(4, 1025, device="cuda"), 4)):
+        with pytest.raises(SeraphError):
+            bad()
+    empty = torch.zeros(0, 8, device="cuda")
+    lp, _, _ = ops.token_logprobs(empty, t[:0])
+    assert lp.numel() == 0
