@@ -184,6 +184,10 @@ int seraph_distill_grad(const float* logits, const uint32_t* teacher_ids, const 
                         int64_t rows, int64_t cols, int64_t top_k, int64_t valid_rows,
                         void* ws, size_t ws_bytes, seraph_stream_t s);
 
+/* What seraph_cross_entropy_exchange_spins is for the cross entropy, for the two ops above whose rows are shared out between
+ * workgroups (policy_grad, distill_grad, beyond 32768 columns). */
+void seraph_objectives_exchange_spins(int spins);
+
 /* ---------------------------------------------------------------- GEMM family */
 /* vulkan_matmul (include/vulkan_backend.h:431-433, shaders/matmul.comp) and
  * vulkan_matmul_transpose (include/vulkan_backend.h:439-442, shaders/matmul_transpose.comp:35-169):

@@ -1,5 +1,7 @@
 // objectives.hip - objectives over vocabulary logits beside the cross entropy: log-probabilities of given tokens, the
 // clipped policy loss, the paired preference loss and distillation from a teacher's top logits.
+#include <atomic>
+
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -28,9 +30,9 @@ __device__ __forceinline__ float grad_at(float z, float m, ExpScale k, const Row
 
 // ---------------------------------------------------------------- the objectives
 // An objective is a struct of its arguments.  dead(): the outputs of a row that is not supervised.  finish(): called by one lane
-// with the statistics of a supervised row; it writes the row's outputs and returns its gradient.  A row's few scalars
-// are formed in 64 bits: (z - m) - log(sum) keeps no more than 24 bits of a difference that a ratio of
-// log-probabilities needs to more than that, and one lane per row costs nothing beside thousands of logits.
+// with the statistics of a supervised row; it writes the row's outputs (where several workgroups call it, one of them) and
+// returns the row's gradient.  A row's log-probability is formed in 64 bits: in FP32 (z - m) - log(sum) keeps 24 bits of a
+// value near 10, of which a difference of two log-probabilities, or a sum of hundreds, needs more.
 struct LogprobsOp {
     static constexpr bool kGrad = false, kList = false;
     Supervision rows;
@@ -44,7 +46,7 @@ struct LogprobsOp {
         if (entropy) entropy[r] = 0.0f;
     }
     template <int EXTRA>
-    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&) const {
+    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&, bool writes = true) const {
         const double log_s = log((double)st.s);
         logp[r] = (float)(((double)zt - (double)st.m) - log_s);
         if (lse) lse[r] = (float)((double)st.m + log_s);
@@ -69,42 +71,38 @@ struct PolicyOp {
         if (entropy_rows) entropy_rows[r] = 0.0f;
     }
     template <int EXTRA>
-    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&) const {
-        const double log_s = log((double)st.s), total = (double)st.s;
+    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&, bool writes = true) const {
+        const double log_s = log_of(st.s);
         const double logp = ((double)zt - (double)st.m) - log_s;
-        const double w = rows.weights ? (double)rows.weights[r] : 1.0;
-        const double adv = (double)advantages[r];
-        const double rho = exp(logp - (double)old_logp[r]);
-        const double free = rho * adv;
-        const double held = fmin(fmax(rho, 1.0 - (double)clip_low), 1.0 + (double)clip_high) * adv;
-        double loss = free > held ? -held : -free;                // NaN takes the second branch of both and stays NaN
-        double slope = free > held ? 0.0 : -free;                 // d loss / d logp
+        const float w = rows.weights ? rows.weights[r] : 1.0f, adv = advantages[r];
+        const float rho = exp_of((float)(logp - (double)old_logp[r]), 0.0f, kUnitScale);
+        const float free = rho * adv;
+        const float held = fminf(fmaxf(rho, 1.0f - clip_low), 1.0f + clip_high) * adv;
+        float loss = free > held ? -held : -free;                 // NaN takes the second branch of both and stays NaN
+        float slope = free > held ? 0.0f : -free;                 // d loss / d logp
         if (ref_logp) {
             const double d = (double)ref_logp[r] - logp;
-            const double em1 = expm1(d);
-            const double kl = em1 - d;
-            if (kl_rows) kl_rows[r] = (float)kl;
+            const float kl = exp_excess(d, exp_of((float)d, 0.0f, kUnitScale));
+            if (kl_rows && writes) kl_rows[r] = kl;
             if (kl_coef != 0.0f) {
-                loss += (double)kl_coef * kl;
-                slope -= (double)kl_coef * em1;
+                loss = fmaf(kl_coef, kl, loss);
+                slope = fmaf(-kl_coef, kl + (float)d, slope);     // e^d - 1
             }
         }
-        const double sc = w * (double)scale;
-        RowGrad g;
-        g.b = 0.0f;
-        double a = -slope * sc / total;
+        const float sc = w * scale, inv_total = 1.0f / st.s;
+        RowGrad g{-slope * sc * inv_total, 0.0f, -slope * sc, rows.targets[r]};
         if (EXTRA == kEntropy) {
-            const double entropy = log_s - (double)st.x / total;
-            if (entropy_rows) entropy_rows[r] = (float)entropy;
-            loss -= (double)entropy_coef * entropy;
-            a += (double)entropy_coef * sc * (entropy - log_s) / total;     // d(-H)/dz_j = p_j (log p_j + H)
-            g.b = (float)((double)entropy_coef * sc / total);
+            const float below = st.x * inv_total;                 // the mean of z - m
+            const float entropy = (float)(log_s - (double)below);
+            if (entropy_rows && writes) entropy_rows[r] = entropy;
+            loss = fmaf(-entropy_coef, entropy, loss);
+            g.b = entropy_coef * sc * inv_total;                  // d(-H)/dz_j = p_j (log p_j + H) = p_j ((z_j - m) - below)
+            g.a -= g.b * below;
         }
-        g.a = (float)a;
-        g.c = (float)(-slope * sc);
-        g.target = rows.targets[r];
-        loss_rows[r] = (float)(w * loss);
-        if (logp_rows) logp_rows[r] = (float)logp;
+        if (writes) {
+            loss_rows[r] = w * loss;
+            if (logp_rows) logp_rows[r] = (float)logp;
+        }
         return g;
     }
 };
@@ -140,33 +138,25 @@ struct DistillOp {
     __device__ __forceinline__ void dead(int64_t r) const { loss_rows[r] = 0.0f; }
     // what an entry with the part q of the teacher's mass takes off the gradient
     __device__ __forceinline__ float entry_scale(int64_t r) const {
-        const double w = rows.weights ? (double)rows.weights[r] : 1.0;
-        return (float)(w * (double)scale * (double)soft_coef * inv_temp);
+        return (rows.weights ? rows.weights[r] : 1.0f) * scale * soft_coef * (float)inv_temp;
     }
     template <int EXTRA>
-    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums& list_sums) const {
-        const double mass = list_sums.mass;
-        const double w = rows.weights ? (double)rows.weights[r] : 1.0;
-        const double sc = w * (double)scale;
-        const int64_t t = target(r);
-        double loss = 0.0, a = 0.0;
-        if (soft_coef != 0.0f && mass != 0.0) {
-            loss = (double)soft_coef * (list_sums.cross + mass * (((double)st.m - (double)list_sums.at) * inv_temp + log((double)st.s)));
-            a = (double)soft_coef * inv_temp * sc * mass / (double)st.s;
+    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums& list_sums, bool writes = true) const {
+        const float w = rows.weights ? rows.weights[r] : 1.0f, sc = w * scale, mass = (float)list_sums.mass;
+        RowGrad g{0.0f, 0.0f, 0.0f, target(r)};
+        double loss = 0.0;
+        if (soft_coef != 0.0f && mass != 0.0f) {
+            loss = (double)soft_coef * (list_sums.cross + list_sums.mass * (((double)st.m - (double)list_sums.at) * inv_temp + log_of(st.s)));
+            g.a = soft_coef * (float)inv_temp * sc * mass / st.s;
         }
-        RowGrad g;
-        g.b = 0.0f;
-        g.c = 0.0f;
-        g.target = t;
-        if (t >= 0) {
-            const double s1 = (double)(EXTRA == kSecond ? st.x : st.s);      // the sum at T = 1
-            loss += (double)hard_coef * (log(s1) - ((double)zt - (double)st.m));
-            if (EXTRA == kSecond) g.b = (float)((double)hard_coef * sc / s1);
-            else a += (double)hard_coef * sc / s1;
-            g.c = (float)((double)hard_coef * sc);
+        if (g.target >= 0) {
+            const float s1 = EXTRA == kSecond ? st.x : st.s;      // the sum at T = 1
+            loss += (double)hard_coef * (log_of(s1) - ((double)zt - (double)st.m));
+            g.c = hard_coef * sc;
+            if (EXTRA == kSecond) g.b = g.c / s1;
+            else g.a += g.c / s1;
         }
-        g.a = (float)a;
-        loss_rows[r] = (float)(w * loss);
+        if (writes) loss_rows[r] = (float)((double)w * loss);
         return g;
     }
 };
@@ -241,6 +231,433 @@ __device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, c
     return sums;
 }
 
+// ---------------------------------------------------------------- rows held in registers
+// One workgroup owns a row of up to 4 kBlock VPT columns (and seven single values) and holds it in its registers: a logit
+// crosses memory once in each direction.
+template <class Op, int EXTRA, int VPT>
+__global__ __launch_bounds__(kBlock) void held_rows_kernel(Op op, const float* logits, float* grad, int cols) {
+    __shared__ float red[3][kBlock / 64];
+    __shared__ RowGrad bcast;
+    __shared__ ListRoom<kBlock, Op::kList ? kMaxTopK : 1> room;
+    const int64_t row = blockIdx.x;
+    const float* x = logits + row * cols;
+    float* out = Op::kGrad ? grad + row * cols : nullptr;
+    const RowShape sh(x, cols);
+    const int single = (int)sh.single((int)threadIdx.x);
+    const SlotBuffer xs(x + sh.head, sh.n4);
+    if (!op.live(row)) {
+        if constexpr (Op::kGrad) {
+            const SlotBuffer gs(out + sh.head, sh.n4);
+#pragma unroll
+            for (int k = 0; k < VPT; k++) gs.store<kNontemporal>(f4{0, 0, 0, 0}, (k * kBlock + (int)threadIdx.x) * 16);
+            if (single >= 0) out[single] = 0.0f;
+        }
+        if (threadIdx.x == 0) op.dead(row);
+        return;
+    }
+    f4 v[VPT];
+#pragma unroll
+    for (int k = 0; k < VPT; k++) v[k] = xs.load<kNontemporal>((k * kBlock + (int)threadIdx.x) * 16);
+    float one = single >= 0 ? x[single] : -INFINITY;
+    float zt = 0.0f;
+    if (threadIdx.x == 0) {
+        const int64_t t = op.target(row);
+        if (t >= 0) zt = x[t];
+    }
+    ListSums sums{0.0, 0.0, 0.0f};
+    if constexpr (Op::kList) sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+    const ExpScale ks = op.k;
+    float m = fmaxf(kLowest, one);
+#pragma unroll
+    for (int k = 0; k < VPT; k++) {
+        if (k * kBlock + (int)threadIdx.x >= sh.n4) v[k] = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
+    }
+    m = block_max<kBlock>(m, red[0]);
+    float e1 = exp_of(one, m, ks), s = e1, ex = EXTRA != kNone ? extra_of<EXTRA>(one, m, e1) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < VPT; k++) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const float e = exp_of(v[k][c], m, ks);
+            s += e;
+            if (EXTRA != kNone) ex += extra_of<EXTRA>(v[k][c], m, e);
+            else if (Op::kGrad) v[k][c] = e;                      // the gradient is a multiple of it
+        }
+    }
+    if (EXTRA != kNone) block_sum2<kBlock>(s, ex, red[1]);
+    else s = block_sum<kBlock>(s, red[1]);
+    if (threadIdx.x == 0) bcast = op.template finish<EXTRA>(row, RowStats{m, s, ex}, zt, sums);
+    if constexpr (Op::kGrad) {
+        __syncthreads();
+        const RowGrad g = bcast;
+        const SlotBuffer gs(out + sh.head, sh.n4);
+        const int tv = (int)g.target - sh.head, t4 = g.target >= sh.head ? tv >> 2 : -1;      // the target's place among the vectors
+        const f4 off_target = {(tv & 3) == 0 ? g.c : 0.0f, (tv & 3) == 1 ? g.c : 0.0f, (tv & 3) == 2 ? g.c : 0.0f, (tv & 3) == 3 ? g.c : 0.0f};
+        // the exponentials are formed again from the logits: kept from the sums they would double the registers of a row
+        if (EXTRA != kNone) asm volatile("" : "+v"(m));
+#pragma unroll
+        for (int k = 0; k < VPT; k++) {
+            const int i4 = k * kBlock + (int)threadIdx.x;
+            f4 r;
+#pragma unroll
+            for (int c = 0; c < 4; c++) r[c] = EXTRA == kNone ? g.a * v[k][c] : grad_at<EXTRA>(v[k][c], m, ks, g);
+            if (t4 == i4) r -= off_target;
+            gs.store<kNontemporal>(r, i4 * 16);
+        }
+        if (single >= 0) {
+            const float r = grad_at<EXTRA>(one, m, ks, g);
+            out[single] = single == g.target ? r - g.c : r;
+        }
+        if constexpr (Op::kList) {
+            const float es = op.entry_scale(row);
+            // the entries' places have been written by other lanes, and those stores are complete before the second ones
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            for (int i = threadIdx.x; i < op.list.top_k; i += kBlock) {
+                const uint32_t id = room.id[i];
+                if ((int64_t)id < cols) out[id] = grad_at<EXTRA>(room.z[i], m, ks, g) - es * room.q[i] - ((int64_t)id == g.target ? g.c : 0.0f);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- long rows shared out between workgroups
+// A row that one workgroup's registers cannot hold is cut into chunks of 4 KB (one vector per lane of a workgroup); chunk c
+// belongs to part c % P, and P workgroups hold one part each, kPartVpt vectors per lane, so that a logit still crosses
+// memory once in each direction.  Each publishes its part's maximum and sums in a record in device memory and combines
+// the row's P records by itself in one fixed order, so all of them arrive at the same bits.
+//
+// The grid is persistent (a multiple of P, at most kPartsPerCu workgroups on a CU); workgroup g takes units g, g + G, ...,
+// unit u being part u % P of row u / P, and loads its next unit's slots as it stores this one's.  A small kernel ahead of this
+// one clears the records (nothing is carried over from another call or from an earlier replay of a captured one) and
+// gathers what belongs to a row as a whole: its target's logit and its list.
+//
+// The wait for a partner's record is bounded.  Past the limit a workgroup forms the missing part's statistics from the
+// logits, with the owner's slots per lane and order of additions, hence to the owner's bits; and if the record has
+// appeared meanwhile it takes that, because in place the owner may by then be overwriting those logits (it
+// publishes before it stores).  So no workgroup ever depends on another one being scheduled.
+constexpr int kPartVpt = 19;                 // 76 of the 128 registers that a lane has with four workgroups on a CU
+constexpr int kPartsPerCu = 4;
+constexpr int kMaxParts = 64;                // one lane of the first wave per partner
+
+// Each word carries its own validity in its upper half, so no order between the words is needed, hence no fence (which
+// at this scope would write back and invalidate whole caches): relaxed device-scope atomics go past the XCDs' L2s.
+struct PartRecord { unsigned long long max_word, sum_word, extra_word, unused; };
+constexpr unsigned long long kPublished = 1ull << 32;
+
+struct RowPrep { ListSums sums; float zt; int live; };
+
+__device__ __forceinline__ void put_word(unsigned long long* w, float v) {
+    __hip_atomic_store(w, kPublished | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <int EXTRA>
+__device__ __forceinline__ bool get_record(PartRecord* rec, RowStats& st) {
+    const unsigned long long a = __hip_atomic_load(&rec->max_word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned long long b = __hip_atomic_load(&rec->sum_word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned long long c = EXTRA == kNone ? kPublished : __hip_atomic_load(&rec->extra_word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const bool ok = (a & b & c & kPublished) != 0;
+    st.m = ok ? __uint_as_float((unsigned)a) : st.m;
+    st.s = ok ? __uint_as_float((unsigned)b) : st.s;
+    st.x = ok ? __uint_as_float((unsigned)c) : st.x;
+    return ok;
+}
+
+// a part's sums against the row's maximum m
+template <int EXTRA>
+__device__ __forceinline__ RowStats against(RowStats st, float m, ExpScale k) {
+    const float r = exp_of(st.m, m, k);
+    RowStats o{m, st.s == 0.0f ? 0.0f : st.s * r, 0.0f};
+    if (EXTRA == kEntropy) o.x = st.s == 0.0f || r == 0.0f ? 0.0f : (st.x + (st.m - m) * st.s) * r;
+    if (EXTRA == kSecond) o.x = st.x == 0.0f ? 0.0f : st.x * exp_of(st.m, m, kUnitScale);
+    return o;
+}
+
+// Clears the row's records and gathers its target's logit; one lane per row, or (rows with lists) one workgroup per row.
+template <class Op>
+__global__ __launch_bounds__(kBlock) void prepare_rows_kernel(Op op, const float* logits, int64_t rows, int64_t cols, int P, RowPrep* prep,
+                                                              PartRecord* records, float* list_q, float* list_z) {
+    if constexpr (Op::kList) {
+        __shared__ ListRoom<kBlock, kMaxTopK> room;
+        const int64_t row = blockIdx.x;
+        unsigned long long* words = reinterpret_cast<unsigned long long*>(records + row * P);
+        for (int i = threadIdx.x; i < P * 4; i += kBlock) __hip_atomic_store(words + i, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const float* x = logits + row * cols;
+        const bool live = op.live(row);
+        RowPrep p{{0.0, 0.0, 0.0f}, 0.0f, live ? 1 : 0};
+        if (live) {
+            p.sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+            for (int i = threadIdx.x; i < op.list.top_k; i += kBlock) {
+                list_q[row * op.list.top_k + i] = room.q[i];
+                list_z[row * op.list.top_k + i] = room.z[i];
+            }
+        }
+        if (threadIdx.x == 0) {
+            const int64_t t = live ? op.target(row) : -1;
+            if (t >= 0) p.zt = x[t];
+            prep[row] = p;
+        }
+    } else {
+        const int64_t row = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+        if (row >= rows) return;
+        unsigned long long* words = reinterpret_cast<unsigned long long*>(records + row * P);
+        for (int i = 0; i < P * 4; i++) __hip_atomic_store(words + i, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool live = op.live(row);
+        const int64_t t = live ? op.target(row) : -1;
+        prep[row] = RowPrep{{0.0, 0.0, 0.0f}, t >= 0 ? logits[row * cols + t] : 0.0f, live ? 1 : 0};
+    }
+}
+
+template <class Op, int EXTRA>
+__global__ __launch_bounds__(kBlock, kPartsPerCu) void shared_rows_kernel(Op op, const float* logits, float* grad, int rows, int64_t cols, int P,
+                                                                          const RowPrep* prep, PartRecord* records, const float* list_q,
+                                                                          const float* list_z, int spin_limit, int in_place) {
+    __shared__ float red[3][kBlock / 64];
+    __shared__ RowStats parts[kMaxParts];
+    __shared__ unsigned long long missing;
+    __shared__ struct { RowGrad g; RowStats st; } bcast;
+    const int part = (int)(blockIdx.x % (unsigned)P), stride = (int)(gridDim.x / (unsigned)P);
+    const ExpScale ks = op.k;
+    const f4 pad = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+
+    // The entries of a list that lie in this part replace what the dense stores left at their places.  Called behind a
+    // barrier that every wave of the workgroup reaches with its stores complete.
+    auto write_entries = [&](int64_t row, const RowGrad& g, float m) {
+        if constexpr (Op::kList) {
+            float* out = grad + row * cols;
+            const int head = RowShape(logits + row * cols, cols).head, n4 = RowShape(logits + row * cols, cols).n4;
+            const float es = op.entry_scale(row);
+            const int64_t base = row * op.list.top_k;
+            for (int i = threadIdx.x; i < op.list.top_k; i += kBlock) {
+                const uint32_t id = op.list.ids[base + i];
+                if ((int64_t)id >= cols) continue;
+                const int i4 = ((int)id - head) >> 2;
+                const int owner = (int)id < head || i4 >= n4 ? 0 : (i4 / kBlock) % P;
+                if (owner == part)
+                    out[id] = grad_at<EXTRA>(list_z[base + i], m, ks, g) - es * list_q[base + i] - ((int64_t)id == g.target ? g.c : 0.0f);
+            }
+        }
+    };
+
+    // A lane's slots lie step_bytes apart.  The offset runs: kept opaque, so that the compiler does not hold one register
+    // per slot over the whole kernel.
+    const int lane_bytes = (part * kBlock + (int)threadIdx.x) * 16, step_bytes = P * kBlock * 16;
+#define SERAPH_NEXT_SLOT(off) do { off += step_bytes; asm volatile("" : "+v"(off)); } while (0)
+    // the next row from r on that is supervised; the rows passed over get their zeros
+    auto next_live = [&](int r) {
+        for (; r < rows && !__builtin_amdgcn_readfirstlane(prep[r].live); r += stride) {
+            float* out = grad + (int64_t)r * cols;
+            const RowShape sh(logits + (int64_t)r * cols, cols);
+            const SlotBuffer gs(out + sh.head, sh.n4);
+            int off = lane_bytes;
+#pragma unroll 1
+            for (int k = 0; k < kPartVpt; k++) { gs.store<kNontemporal>(f4{0, 0, 0, 0}, off); off += step_bytes; }
+            const int64_t single = part == 0 ? sh.single((int)threadIdx.x) : -1;
+            if (single >= 0) out[single] = 0.0f;
+            if (part == 0 && threadIdx.x == 0) op.dead(r);
+        }
+        return r;
+    };
+    int row = next_live((int)(blockIdx.x / (unsigned)P));
+    if (row >= rows) return;
+    f4 v[kPartVpt];
+    float one;
+    {
+        const float* x = logits + (int64_t)row * cols;
+        const RowShape sh(x, cols);
+        const SlotBuffer xs(x + sh.head, sh.n4);
+        int off = lane_bytes;
+#pragma unroll
+        for (int k = 0; k < kPartVpt; k++) { v[k] = xs.load<kNontemporal>(off); SERAPH_NEXT_SLOT(off); }
+        const int64_t c = part == 0 ? sh.single((int)threadIdx.x) : -1;
+        one = c >= 0 ? x[c] : -INFINITY;
+    }
+    for (int listed = -1;;) {                                     // listed: a row whose entries are still to be written
+        const float* x = logits + (int64_t)row * cols;
+        float* out = grad + (int64_t)row * cols;
+        const RowShape sh(x, cols);
+        float m = fmaxf(kLowest, one);
+        {
+            const int end = sh.n4 * 16;
+            int off = lane_bytes;
+#pragma unroll
+            for (int k = 0; k < kPartVpt; k++) {
+                if (off >= end) v[k] = pad;
+                m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
+                SERAPH_NEXT_SLOT(off);
+            }
+        }
+        if (Op::kList) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        RowStats mine{block_max<kBlock>(m, red[0]), 0.0f, 0.0f};
+        if (Op::kList && listed >= 0) write_entries(listed, bcast.g, bcast.st.m);
+        const float e1 = exp_of(one, mine.m, ks);
+        float s = e1, ex = EXTRA != kNone ? extra_of<EXTRA>(one, mine.m, e1) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPartVpt; k++) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const float e = exp_of(v[k][c], mine.m, ks);
+                s += e;
+                if (EXTRA != kNone) ex += extra_of<EXTRA>(v[k][c], mine.m, e);
+                else v[k][c] = e;
+            }
+            asm volatile("" : "+v"(v[k]));                        // four exponentials stay the four registers that a store takes
+        }
+        if (EXTRA != kNone) block_sum2<kBlock>(s, ex, red[1]);
+        else s = block_sum<kBlock>(s, red[1]);
+        mine.s = s;
+        mine.x = ex;
+
+        // The first wave, one lane per part, waits for the row's records (once more, over `parts`, where one was missing).
+        PartRecord* recs = records + (int64_t)row * P;
+        for (bool again = false;; again = true) {
+            if (threadIdx.x < 64) {
+                const int lane = (int)threadIdx.x;
+                RowStats got{kLowest, 0.0f, 0.0f};
+                bool ok = lane >= P;
+                if (!again) {
+                    if (lane == 0) {
+                        put_word(&recs[part].max_word, mine.m);
+                        put_word(&recs[part].sum_word, mine.s);
+                        if (EXTRA != kNone) put_word(&recs[part].extra_word, mine.x);
+                        // in place this part's logits are about to be overwritten: the record is out before that
+                        if (in_place) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    }
+                    if (!ok) ok = get_record<EXTRA>(recs + lane, got);
+                    for (int spin = 0; !ok && spin < spin_limit; spin++) {
+                        __builtin_amdgcn_s_sleep(4);
+                        ok = get_record<EXTRA>(recs + lane, got);
+                    }
+                } else if (!ok) {
+                    got = parts[lane];
+                    ok = true;
+                }
+                const unsigned long long todo = __ballot(!ok);
+                if (lane == 0) missing = todo;
+                if (todo) {
+                    if (lane < P) parts[lane] = got;
+                } else {
+                    const float rm = wave_max(got.m);
+                    const RowStats o = against<EXTRA>(got, rm, ks);
+                    const RowStats total{rm, wave_sum(o.s), EXTRA != kNone ? wave_sum(o.x) : 0.0f};
+                    if (lane == 0) {
+                        bcast.st = total;
+                        bcast.g = op.template finish<EXTRA>(row, total, prep[row].zt, prep[row].sums, part == 0);
+                    }
+                }
+            }
+            __syncthreads();
+            unsigned long long todo = missing;                    // the same value for the whole workgroup
+            if (!todo) break;
+            const SlotBuffer xs(x + sh.head, sh.n4);
+            while (todo) {
+                const int p = __builtin_ctzll(todo);
+                todo &= todo - 1;
+                const int64_t c1 = p == 0 ? sh.single((int)threadIdx.x) : -1;
+                const float o1 = c1 >= 0 ? x[c1] : -INFINITY;
+                float pm = fmaxf(kLowest, o1);
+                __syncthreads();                                  // red and missing have been read
+#pragma unroll 1
+                for (int k = 0; k < kPartVpt; k++) {
+                    const int i4 = (p + k * P) * kBlock + (int)threadIdx.x;
+                    const f4 w = i4 < sh.n4 ? xs.load<0>(i4 * 16) : pad;
+                    pm = fmaxf(pm, fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)));
+                }
+                RowStats st{block_max<kBlock>(pm, red[0]), 0.0f, 0.0f};
+                const float f1 = exp_of(o1, st.m, ks);
+                float ps = f1, px = EXTRA != kNone ? extra_of<EXTRA>(o1, st.m, f1) : 0.0f;
+#pragma unroll 1
+                for (int k = 0; k < kPartVpt; k++) {
+                    const int i4 = (p + k * P) * kBlock + (int)threadIdx.x;
+                    const f4 w = i4 < sh.n4 ? xs.load<0>(i4 * 16) : pad;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const float e = exp_of(w[c], st.m, ks);
+                        ps += e;
+                        if (EXTRA != kNone) px += extra_of<EXTRA>(w[c], st.m, e);
+                    }
+                }
+                if (EXTRA != kNone) block_sum2<kBlock>(ps, px, red[1]);
+                else ps = block_sum<kBlock>(ps, red[1]);
+                st.s = ps;
+                st.x = px;
+                if (threadIdx.x == 0) {                           // (behind the reductions' barriers every lane's loads have returned)
+                    get_record<EXTRA>(recs + p, st);
+                    parts[p] = st;
+                }
+            }
+            __syncthreads();
+        }
+        const RowGrad g = bcast.g;
+        float rm = bcast.st.m;
+        if (EXTRA != kNone) asm volatile("" : "+v"(rm));          // form the exponentials again rather than keep both
+        const float back = EXTRA == kNone ? g.a * exp_of(mine.m, rm, ks) : 0.0f;
+        const int tv = (int)g.target - sh.head, target_bytes = g.target >= sh.head ? (tv >> 2) * 16 : -1;
+        const f4 off_target = {(tv & 3) == 0 ? g.c : 0.0f, (tv & 3) == 1 ? g.c : 0.0f, (tv & 3) == 2 ? g.c : 0.0f, (tv & 3) == 3 ? g.c : 0.0f};
+        const int64_t single = part == 0 ? sh.single((int)threadIdx.x) : -1;
+        if (single >= 0) {
+            const float r = grad_at<EXTRA>(one, rm, ks, g);
+            out[single] = single == g.target ? r - g.c : r;
+        }
+        const int next = next_live(row + stride);
+        const float* xn = logits + (int64_t)(next < rows ? next : row) * cols;
+        const RowShape shn(xn, cols);
+        const SlotBuffer gs(out + sh.head, sh.n4), xs(xn + shn.head, next < rows ? shn.n4 : 0);   // (no slots: loads of nothing)
+        int off = lane_bytes;
+#pragma unroll
+        for (int k = 0; k < kPartVpt; k++) {
+            f4 r;
+#pragma unroll
+            for (int c = 0; c < 4; c++) r[c] = EXTRA == kNone ? back * v[k][c] : grad_at<EXTRA>(v[k][c], rm, ks, g);
+            if (target_bytes == off) r -= off_target;
+            gs.store<kNontemporal>(r, off);
+            v[k] = xs.load<kNontemporal>(off);
+            SERAPH_NEXT_SLOT(off);
+        }
+        listed = row;
+        if (next >= rows) break;
+        row = next;
+        const int64_t c = part == 0 ? shn.single((int)threadIdx.x) : -1;
+        one = c >= 0 ? xn[c] : -INFINITY;
+    }
+    if constexpr (Op::kList) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        write_entries(row, bcast.g, bcast.st.m);
+    }
+#undef SERAPH_NEXT_SLOT
+}
+
+static int shared_parts(int64_t cols) { return (int)ceil_div(ceil_div(cols / 4, kBlock), kPartVpt); }
+static bool is_shared(int64_t cols) { return cols > 32768 && shared_parts(cols) <= kMaxParts; }
+static inline size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+static size_t shared_ws_bytes(int64_t rows, int64_t cols, int64_t top_k) {
+    if (rows <= 0 || cols <= 0 || !is_shared(cols)) return 0;
+    return up16((size_t)rows * sizeof(RowPrep)) + (size_t)rows * shared_parts(cols) * sizeof(PartRecord) + 2 * up16((size_t)rows * (size_t)(top_k > 0 ? top_k : 0) * 4);
+}
+
+static std::atomic<int> g_spin_limit{1 << 16};                    // waits of ~0.3 us each
+
+template <class Op, int EXTRA>
+static int launch_shared(const Op& op, const float* logits, float* grad, int64_t rows, int64_t cols, int64_t top_k, void* ws, hipStream_t st) {
+    const int P = shared_parts(cols);
+    char* p = reinterpret_cast<char*>(ws);
+    RowPrep* prep = reinterpret_cast<RowPrep*>(p);
+    PartRecord* records = reinterpret_cast<PartRecord*>(p += up16((size_t)rows * sizeof(RowPrep)));
+    float* list_q = reinterpret_cast<float*>(p += (size_t)rows * P * sizeof(PartRecord));
+    float* list_z = reinterpret_cast<float*>(p += up16((size_t)rows * (size_t)top_k * 4));
+    const unsigned prep_grid = Op::kList ? (unsigned)rows : (unsigned)ceil_div(rows, kBlock);
+    hipLaunchKernelGGL((prepare_rows_kernel<Op>), dim3(prep_grid), dim3(kBlock), 0, st, op, logits, rows, cols, P, prep, records, list_q, list_z);
+    SERAPH_LAUNCH_CHECK();
+    int64_t G = (int64_t)num_compute_units() * kPartsPerCu / P * P;
+    if (G < P) G = P;
+    if (G > rows * P) G = rows * P;
+    hipLaunchKernelGGL((shared_rows_kernel<Op, EXTRA>), dim3((unsigned)G), dim3(kBlock), 0, st, op, logits, grad, (int)rows, cols, P, prep, records,
+                       list_q, list_z, g_spin_limit.load(), grad == logits ? 1 : 0);
+    SERAPH_LAUNCH_CHECK();
+    return SERAPH_OK;
+}
+
 // ---------------------------------------------------------------- rows swept from memory
 // One workgroup per row: maximum, sums, gradient, each a sweep of its own.
 template <class Op, int EXTRA>
@@ -294,7 +711,22 @@ __global__ __launch_bounds__(kBlock) void swept_rows_kernel(Op op, const float* 
 }
 
 template <class Op, int EXTRA>
-static int launch_rows(const Op& op, const float* logits, float* grad, int64_t rows, int64_t cols, hipStream_t st) {
+static int launch_rows(const Op& op, const float* logits, float* grad, int64_t rows, int64_t cols, int64_t top_k, void* ws, hipStream_t st) {
+    if (cols <= 32768) {
+        const int64_t n4 = cols / 4;
+#define HELD(V) hipLaunchKernelGGL((held_rows_kernel<Op, EXTRA, V>), dim3((unsigned)rows), dim3(kBlock), 0, st, op, logits, grad, (int)cols)
+        if (n4 <= 1 * kBlock) HELD(1);
+        else if (n4 <= 2 * kBlock) HELD(2);
+        else if (n4 <= 4 * kBlock) HELD(4);
+        else if (n4 <= 8 * kBlock) HELD(8);
+        else if (n4 <= 16 * kBlock) HELD(16);
+        else HELD(32);
+#undef HELD
+        SERAPH_LAUNCH_CHECK();
+        return SERAPH_OK;
+    }
+    if constexpr (Op::kGrad)
+        if (is_shared(cols)) return launch_shared<Op, EXTRA>(op, logits, grad, rows, cols, top_k, ws, st);
     hipLaunchKernelGGL((swept_rows_kernel<Op, EXTRA>), dim3((unsigned)rows), dim3(kBlock), 0, st, op, logits, grad, cols);
     SERAPH_LAUNCH_CHECK();
     return SERAPH_OK;
@@ -333,7 +765,7 @@ struct PairRowsOp {
         if (logp_rows) logp_rows[r] = 0.0f;
     }
     template <int EXTRA>
-    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&) const {
+    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&, bool writes = true) const {
         const double v = ((double)zt - (double)st.m) - log((double)st.s);
         totals[r] = RowTotals{st.m, st.s};
         factors[r] = RowFactor{st.m, 0.0f, 0.0f, rows.targets[r]};
@@ -411,8 +843,6 @@ __global__ __launch_bounds__(kBlock) void pair_grad_kernel(const float* logits, 
     }
 }
 
-static inline size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
-
 }  // namespace seraph
 
 using namespace seraph;
@@ -430,6 +860,10 @@ using namespace seraph;
 
 extern "C" {
 
+void seraph_objectives_exchange_spins(int spins) {
+    if (spins >= 0) g_spin_limit = spins;
+}
+
 size_t seraph_token_logprobs_ws_bytes(int64_t rows, int64_t cols) {
     (void)rows; (void)cols;
     return 0;
@@ -444,14 +878,11 @@ int seraph_token_logprobs(const float* logits, const uint32_t* targets, float* l
     SERAPH_REQUIRE(!seq_starts || batch >= 1, "token_logprobs: packed call needs batch >= 1");
     REQUIRE_WS("token_logprobs", seraph_token_logprobs_ws_bytes(rows, cols));
     LogprobsOp op{{targets, nullptr, seq_starts, batch, cols}, logp, lse, entropy, kUnitScale};
-    if (entropy) return launch_rows<LogprobsOp, kEntropy>(op, logits, nullptr, rows, cols, as_stream(s));
-    return launch_rows<LogprobsOp, kNone>(op, logits, nullptr, rows, cols, as_stream(s));
+    if (entropy) return launch_rows<LogprobsOp, kEntropy>(op, logits, nullptr, rows, cols, 0, ws, as_stream(s));
+    return launch_rows<LogprobsOp, kNone>(op, logits, nullptr, rows, cols, 0, ws, as_stream(s));
 }
 
-size_t seraph_policy_grad_ws_bytes(int64_t rows, int64_t cols) {
-    (void)rows; (void)cols;
-    return 0;
-}
+size_t seraph_policy_grad_ws_bytes(int64_t rows, int64_t cols) { return shared_ws_bytes(rows, cols, 0); }
 
 int seraph_policy_grad(const float* logits, const uint32_t* actions, const float* advantages, const float* old_logp,
                        const float* ref_logp, const float* weights, float* grad, float* loss_rows,
@@ -470,8 +901,8 @@ int seraph_policy_grad(const float* logits, const uint32_t* actions, const float
     const float scale = valid_rows > 0 ? 1.0f / (float)valid_rows : 0.0f;
     PolicyOp op{{actions, weights, seq_starts, batch, cols}, advantages, old_logp, ref_logp, loss_rows, logp_rows, kl_rows, entropy_rows,
                 options->clip_low, options->clip_high, options->kl_coef, options->entropy_coef, scale, kUnitScale};
-    if (options->entropy_coef != 0.0f || entropy_rows) return launch_rows<PolicyOp, kEntropy>(op, logits, grad, rows, cols, as_stream(s));
-    return launch_rows<PolicyOp, kNone>(op, logits, grad, rows, cols, as_stream(s));
+    if (options->entropy_coef != 0.0f || entropy_rows) return launch_rows<PolicyOp, kEntropy>(op, logits, grad, rows, cols, 0, ws, as_stream(s));
+    return launch_rows<PolicyOp, kNone>(op, logits, grad, rows, cols, 0, ws, as_stream(s));
 }
 
 size_t seraph_preference_grad_ws_bytes(int64_t rows, int64_t cols) {
@@ -498,7 +929,7 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
     double* logp = reinterpret_cast<double*>(p += up16((size_t)rows * sizeof(RowFactor)));
     RowTotals* totals = reinterpret_cast<RowTotals*>(p += up16((size_t)rows * sizeof(double)));
     PairRowsOp op{{targets, nullptr, seq_starts, 2 * pairs, cols}, totals, logp, factors, logp_rows, kUnitScale};
-    const int rc = launch_rows<PairRowsOp, kNone>(op, logits, nullptr, rows, cols, st);
+    const int rc = launch_rows<PairRowsOp, kNone>(op, logits, nullptr, rows, cols, 0, ws, st);
     if (rc != SERAPH_OK) return rc;
     PreferenceArgs a{ref_logp, loss_pairs, scores, logp_rows, seq_starts, pairs, rows, options->kind, options->average,
                      options->beta, options->label_smoothing, options->margin};
@@ -509,10 +940,7 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
     return SERAPH_OK;
 }
 
-size_t seraph_distill_grad_ws_bytes(int64_t rows, int64_t cols, int64_t top_k) {
-    (void)rows; (void)cols; (void)top_k;
-    return 0;
-}
+size_t seraph_distill_grad_ws_bytes(int64_t rows, int64_t cols, int64_t top_k) { return shared_ws_bytes(rows, cols, top_k); }
 
 int seraph_distill_grad(const float* logits, const uint32_t* teacher_ids, const void* teacher_logits, const float* teacher_lse,
                         const uint32_t* targets, const float* weights, float* grad, float* loss_rows,
@@ -534,8 +962,8 @@ int seraph_distill_grad(const float* logits, const uint32_t* teacher_ids, const 
     DistillOp op{{nullptr, weights, seq_starts, batch, cols}, {teacher_ids, teacher_logits, teacher_lse, options->teacher_type, (int)top_k},
                  targets, loss_rows, options->soft_coef, options->hard_coef, scale, ExpScale::of(1.0 / (double)options->temperature), 1.0 / (double)options->temperature};
     // at T = 1 the two parts share their exponentials
-    if (options->hard_coef != 0.0f && options->temperature != 1.0f) return launch_rows<DistillOp, kSecond>(op, logits, grad, rows, cols, as_stream(s));
-    return launch_rows<DistillOp, kNone>(op, logits, grad, rows, cols, as_stream(s));
+    if (options->hard_coef != 0.0f && options->temperature != 1.0f) return launch_rows<DistillOp, kSecond>(op, logits, grad, rows, cols, top_k, ws, as_stream(s));
+    return launch_rows<DistillOp, kNone>(op, logits, grad, rows, cols, top_k, ws, as_stream(s));
 }
 
 }  // extern "C"

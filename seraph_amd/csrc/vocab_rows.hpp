@@ -47,6 +47,28 @@ __device__ __forceinline__ float exp_of(float z, float m, ExpScale k) {
     return __builtin_amdgcn_exp2f(fmaf(d, k.hi, d * k.lo));
 }
 
+// log s in 64 bits, off by 1e-7 at most: the exponent is exact, the logarithm of the mantissa lies in [-ln 2, 0].  A few
+// instructions and registers, where log(double) needs dozens of both beside a row that fills a lane's registers.
+__device__ __forceinline__ double log_of(float s) {
+    return (double)__builtin_amdgcn_frexp_expf(s) * 0.693147180559945309 + (double)(__builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(s)) * 0.6931471805599453f);
+}
+
+// e^d - 1 - d to a few units of its last place, d >= 0 or d < 0: the series where the three would cancel.
+__device__ __forceinline__ float exp_excess(double d, float e) {
+    if (fabs(d) >= 1.0) return (float)((double)e - 1.0 - d);
+    const float x = (float)d;
+    float p = 1.0f / 3628800.0f;                                  // x^2 (1/2! + x/3! + ... + x^8/10!)
+    p = fmaf(p, x, 1.0f / 362880.0f);
+    p = fmaf(p, x, 1.0f / 40320.0f);
+    p = fmaf(p, x, 1.0f / 5040.0f);
+    p = fmaf(p, x, 1.0f / 720.0f);
+    p = fmaf(p, x, 1.0f / 120.0f);
+    p = fmaf(p, x, 1.0f / 24.0f);
+    p = fmaf(p, x, 1.0f / 6.0f);
+    p = fmaf(p, x, 0.5f);
+    return x * x * p;
+}
+
 template <int EXTRA>
 __device__ __forceinline__ float extra_of(float z, float m, float e) {
     if (EXTRA == kEntropy) return e > 0.0f ? e * (z - m) : (e == 0.0f ? 0.0f : e);      // exp(-inf) (-inf) counts 0, NaN stays
@@ -75,6 +97,22 @@ __device__ __forceinline__ T block_sum(T v, T* lds) {
     return r;
 }
 
+// both sums over the workgroup behind one barrier; lds holds 2 BLOCK / 64 floats
+template <int BLOCK>
+__device__ __forceinline__ void block_sum2(float& a, float& b, float* lds) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if ((threadIdx.x & 63) == 0) {
+        lds[threadIdx.x >> 6] = a;
+        lds[BLOCK / 64 + (threadIdx.x >> 6)] = b;
+    }
+    __syncthreads();
+    a = lds[0];
+    b = lds[BLOCK / 64];
+#pragma unroll
+    for (int w = 1; w < BLOCK / 64; w++) { a += lds[w]; b += lds[BLOCK / 64 + w]; }
+}
+
 // A row of floats that need not start on a 16-byte boundary nor hold a multiple of four: `head` single values up to the
 // first boundary, n4 vectors, `tail` single values.  Lanes 0..3 of one workgroup hold the head, lanes 4..7 the tail.
 struct RowShape {
@@ -90,6 +128,27 @@ struct RowShape {
         if (lane < head) return lane;
         if (lane >= 4 && lane < 4 + tail) return (int64_t)head + (int64_t)n4 * 4 + (lane - 4);
         return -1;
+    }
+};
+
+// The vectors of a row as a buffer of n4 16-byte slots: a scalar descriptor and one 32-bit offset per lane.  A load past the
+// last slot returns zeros and a store past it is dropped, so a slot needs no branch.  The offset is the lane's alone (no scalar
+// offset), which is what the range check compares; the address itself may be any multiple of four.
+constexpr int kNontemporal = 2;
+struct SlotBuffer {
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ __forceinline__ SlotBuffer(const float* first, int n4) {
+        const uint64_t o = reinterpret_cast<uint64_t>(first);
+        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)o), hi = __builtin_amdgcn_readfirstlane((uint32_t)(o >> 32));
+        rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(n4 * 16), 0x00020000);
+    }
+    template <int AUX>
+    __device__ __forceinline__ f4 load(int offset) const {
+        return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, offset, 0, AUX));
+    }
+    template <int AUX>
+    __device__ __forceinline__ void store(f4 v, int offset) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(__attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned, v), rsrc, offset, 0, AUX);
     }
 };
 

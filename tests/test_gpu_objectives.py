@@ -328,7 +328,7 @@ def test_many_rows_and_one(ops, rows, cols):
     hot = torch.zeros_like(p).scatter_(1, t.long()[:, None], 1.0)
     f = (2.0 / rows) * rho[:, None]
     assert ((grad.double() - f * (p - hot)).abs() <= 4 * u * f * (p + hot)).all()
-    assert torch.equal(lp, logp)
+    assert ((lp.double() - want).abs() <= u + ref.HALF_STEP * want.abs()).all()
     k = 5
     ids = torch.stack([torch.randperm(cols, device="cuda", generator=g)[:k] for _ in range(rows)]).to(torch.int32)
     tl = torch.empty(rows, k, device="cuda").normal_(generator=g)
@@ -431,6 +431,34 @@ def test_two_streams_at_once(ops):
     torch.cuda.synchronize()
     for i, res in enumerate(got):
         assert all(x is None or torch.equal(x, y) for x, y in zip(res, alone[i % 2]))
+
+
+@pytest.mark.parametrize("rows,cols", [(5, 40001), (700, 65536), (3, 1200000)])
+@pytest.mark.parametrize("spins", [0, 1])
+def test_long_rows_when_partners_are_not_waited_for(ops, rows, cols, spins):
+    """Whoever learns a part's statistics in whichever way, the bits are the same; in place too."""
+    from seraph_amd._lib import kernels
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    z = torch.empty(rows, cols, device="cuda").normal_(0, 2, generator=g)
+    t = torch.randint(0, cols, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    t[1] = -1
+    old, adv = torch.full((rows,), -11.0, device="cuda"), torch.ones(rows, device="cuda")
+    ids = torch.randint(0, cols + 9, (rows, 33), device="cuda", generator=g, dtype=torch.int32)
+    tl = torch.empty(rows, 33, device="cuda").normal_(generator=g)
+    calls = [lambda x, out: ops.policy_grad(x, t, adv, old, rows, ref_logp=old, kl_coef=0.1, grad=out),
+             lambda x, out: ops.policy_grad(x, t, adv, old, rows, entropy_coef=0.1, grad=out),
+             lambda x, out: ops.distill_grad(x, ids, tl, rows, grad=out),
+             lambda x, out: ops.distill_grad(x, ids, tl, rows, temperature=2.0, hard_coef=0.5, targets=t, grad=out)]
+    for call in calls:
+        want = call(z, None)
+        try:
+            kernels().seraph_objectives_exchange_spins(spins)
+            for x in (z, z.clone()):
+                got = call(x, None if x is z else x)
+                torch.cuda.synchronize()
+                assert all(a is None or torch.equal(a, b) for a, b in zip(got, want))
+        finally:
+            kernels().seraph_objectives_exchange_spins(1 << 16)
 
 
 def test_wrapper_refusals(ops):
