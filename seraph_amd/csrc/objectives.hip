@@ -658,17 +658,120 @@ static int launch_shared(const Op& op, const float* logits, float* grad, int64_t
     return SERAPH_OK;
 }
 
+// ---------------------------------------------------------------- long rows read once
+// Forward only: nothing has to be held.  A row is cut into `splits` runs of vectors, each streamed by one workgroup that keeps
+// a running maximum and sums per lane; one wave per row then puts the runs' results together.  Splitting serves
+// few rows, which alone would leave most of the chip idle, and evens out the last round of many.
+template <int EXTRA>
+__device__ __forceinline__ void add_logit(RowStats& st, float z, ExpScale k) {
+    const float e = exp_of(z, st.m, k);
+    st.s += e;
+    if (EXTRA != kNone) st.x += extra_of<EXTRA>(z, st.m, e);
+}
+
+template <class Op, int EXTRA>
+__global__ __launch_bounds__(kBlock) void streamed_rows_kernel(Op op, const float* logits, int64_t cols, int splits, RowStats* runs) {
+    constexpr int kAhead = 8;                                     // vectors in flight per lane
+    __shared__ float red[3][kBlock / 64];
+    const int64_t row = blockIdx.x / (unsigned)splits;
+    const int run = (int)(blockIdx.x % (unsigned)splits);
+    if (!op.live(row)) return;
+    const float* x = logits + row * cols;
+    const RowShape sh(x, cols);
+    const f4* xv = reinterpret_cast<const f4*>(x + sh.head);
+    const int per_run = ((sh.n4 + splits - 1) / splits + kBlock - 1) / kBlock * kBlock;
+    const int first = run * per_run, end = first + per_run < sh.n4 ? first + per_run : sh.n4;
+    const ExpScale ks = op.k;
+    RowStats st{kLowest, 0.0f, 0.0f};
+    auto raise = [&](float m) {                                   // a new running maximum
+        if (m > st.m) {
+            st = against<EXTRA>(st, m, ks);
+            st.m = m;
+        }
+    };
+    int i4 = first + (int)threadIdx.x;
+    for (; i4 + (kAhead - 1) * kBlock < end; i4 += kAhead * kBlock) {
+        f4 v[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) v[j] = __builtin_nontemporal_load(xv + i4 + j * kBlock);
+        float m = kLowest;
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) m = fmaxf(m, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
+        raise(m);
+#pragma unroll
+        for (int j = 0; j < kAhead; j++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) add_logit<EXTRA>(st, v[j][c], ks);
+    }
+    for (; i4 < end; i4 += kBlock) {
+        const f4 v = __builtin_nontemporal_load(xv + i4);
+        raise(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+#pragma unroll
+        for (int c = 0; c < 4; c++) add_logit<EXTRA>(st, v[c], ks);
+    }
+    const int64_t single = run == 0 ? sh.single((int)threadIdx.x) : -1;
+    if (single >= 0) {
+        const float z = x[single];
+        raise(z);
+        add_logit<EXTRA>(st, z, ks);
+    }
+    const float m = block_max<kBlock>(st.m, red[0]);
+    RowStats o = against<EXTRA>(st, m, ks);
+    if (EXTRA != kNone) block_sum2<kBlock>(o.s, o.x, red[1]);
+    else o.s = block_sum<kBlock>(o.s, red[1]);
+    if (threadIdx.x == 0) runs[row * splits + run] = RowStats{m, o.s, o.x};
+}
+
+template <class Op, int EXTRA>
+__global__ __launch_bounds__(kBlock) void join_runs_kernel(Op op, const float* logits, int64_t rows, int64_t cols, int splits, const RowStats* runs) {
+    const int64_t row = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
+    const int lane = (int)threadIdx.x & 63;
+    if (row >= rows) return;
+    if (!op.live(row)) {
+        if (lane == 0) op.dead(row);
+        return;
+    }
+    const RowStats got = lane < splits ? runs[row * splits + lane] : RowStats{kLowest, 0.0f, 0.0f};
+    const float m = wave_max(got.m);
+    const RowStats o = against<EXTRA>(got, m, op.k);
+    const RowStats total{m, wave_sum(o.s), EXTRA != kNone ? wave_sum(o.x) : 0.0f};
+    if (lane == 0) op.template finish<EXTRA>(row, total, logits[row * cols + op.target(row)], ListSums{0.0, 0.0, 0.0f});
+}
+
+constexpr int kMaxRuns = 64;
+static int streamed_runs(int64_t rows, int64_t cols) {
+    const int64_t wanted = ceil_div(8192, rows), most = cols / 4 / (8 * kBlock);      // a run has eight vectors per lane at least
+    const int64_t n = wanted < most ? wanted : most;
+    return (int)(n < 1 ? 1 : n > kMaxRuns ? kMaxRuns : n);
+}
+static size_t streamed_ws_bytes(int64_t rows, int64_t cols) {
+    return rows > 0 && cols > 32768 ? up16((size_t)rows * streamed_runs(rows, cols) * sizeof(RowStats)) : 0;
+}
+
+template <class Op, int EXTRA>
+static int launch_streamed(const Op& op, const float* logits, int64_t rows, int64_t cols, void* ws, hipStream_t st) {
+    const int splits = streamed_runs(rows, cols);
+    RowStats* runs = reinterpret_cast<RowStats*>(ws);
+    SERAPH_REQUIRE(rows * splits <= 0x7fffffff, "too many rows: %lld", (long long)rows);
+    hipLaunchKernelGGL((streamed_rows_kernel<Op, EXTRA>), dim3((unsigned)(rows * splits)), dim3(kBlock), 0, st, op, logits, cols, splits, runs);
+    SERAPH_LAUNCH_CHECK();
+    hipLaunchKernelGGL((join_runs_kernel<Op, EXTRA>), dim3((unsigned)ceil_div(rows, kBlock / 64)), dim3(kBlock), 0, st, op, logits, rows, cols, splits, runs);
+    SERAPH_LAUNCH_CHECK();
+    return SERAPH_OK;
+}
+
 // ---------------------------------------------------------------- rows swept from memory
-// One workgroup per row: maximum, sums, gradient, each a sweep of its own.
+// One workgroup per row: maximum, sums, gradient, each a sweep of its own, for rows beyond what kMaxParts workgroups hold
+// (1245184 columns).
 template <class Op, int EXTRA>
 __global__ __launch_bounds__(kBlock) void swept_rows_kernel(Op op, const float* logits, float* grad, int64_t cols) {
     __shared__ float red[3][kBlock / 64];
     __shared__ RowGrad bcast;
     __shared__ ListRoom<kBlock, Op::kList ? kMaxTopK : 1> room;
     const int64_t row = blockIdx.x;
-    float* out = Op::kGrad ? grad + row * cols : nullptr;
+    float* out = grad + row * cols;
     if (!op.live(row)) {
-        if (Op::kGrad) for (int64_t c = threadIdx.x; c < cols; c += kBlock) out[c] = 0.0f;
+        for (int64_t c = threadIdx.x; c < cols; c += kBlock) out[c] = 0.0f;
         if (threadIdx.x == 0) op.dead(row);
         return;
     }
@@ -693,19 +796,17 @@ __global__ __launch_bounds__(kBlock) void swept_rows_kernel(Op op, const float* 
         bcast = op.template finish<EXTRA>(row, st, t >= 0 ? x[t] : 0.0f, sums);
     }
     __syncthreads();
-    if constexpr (Op::kGrad) {
-        const RowGrad g = bcast;
-        for (int64_t c = threadIdx.x; c < cols; c += kBlock) {
-            const float v = grad_at<EXTRA>(x[c], st.m, k, g);
-            out[c] = c == g.target ? v - g.c : v;
-        }
-        if constexpr (Op::kList) {
-            const float es = op.entry_scale(row);
-            __syncthreads();                                      // the sweep has written every entry's place
-            for (int i = threadIdx.x; i < op.list.top_k; i += kBlock) {
-                const uint32_t id = room.id[i];
-                if ((int64_t)id < cols) out[id] = grad_at<EXTRA>(room.z[i], st.m, k, g) - es * room.q[i] - ((int64_t)id == g.target ? g.c : 0.0f);
-            }
+    const RowGrad g = bcast;
+    for (int64_t c = threadIdx.x; c < cols; c += kBlock) {
+        const float v = grad_at<EXTRA>(x[c], st.m, k, g);
+        out[c] = c == g.target ? v - g.c : v;
+    }
+    if constexpr (Op::kList) {
+        const float es = op.entry_scale(row);
+        __syncthreads();                                          // the sweep has written every entry's place
+        for (int i = threadIdx.x; i < op.list.top_k; i += kBlock) {
+            const uint32_t id = room.id[i];
+            if ((int64_t)id < cols) out[id] = grad_at<EXTRA>(room.z[i], st.m, k, g) - es * room.q[i] - ((int64_t)id == g.target ? g.c : 0.0f);
         }
     }
 }
@@ -725,11 +826,14 @@ static int launch_rows(const Op& op, const float* logits, float* grad, int64_t r
         SERAPH_LAUNCH_CHECK();
         return SERAPH_OK;
     }
-    if constexpr (Op::kGrad)
+    if constexpr (Op::kGrad) {
         if (is_shared(cols)) return launch_shared<Op, EXTRA>(op, logits, grad, rows, cols, top_k, ws, st);
-    hipLaunchKernelGGL((swept_rows_kernel<Op, EXTRA>), dim3((unsigned)rows), dim3(kBlock), 0, st, op, logits, grad, cols);
-    SERAPH_LAUNCH_CHECK();
-    return SERAPH_OK;
+        hipLaunchKernelGGL((swept_rows_kernel<Op, EXTRA>), dim3((unsigned)rows), dim3(kBlock), 0, st, op, logits, grad, cols);
+        SERAPH_LAUNCH_CHECK();
+        return SERAPH_OK;
+    } else {
+        return launch_streamed<Op, EXTRA>(op, logits, rows, cols, ws, st);
+    }
 }
 
 // ---------------------------------------------------------------- preference pairs
@@ -828,18 +932,48 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PreferenceArgs p, const Ro
     }
 }
 
-__global__ __launch_bounds__(kBlock) void pair_grad_kernel(const float* logits, float* grad, const RowFactor* factors, int64_t cols) {
-    const int64_t row = blockIdx.x;
+// One workgroup per run of kPairVpt vectors per lane of a row; the rows are walked back from the last one, whose logits the
+// pass before this one has left in the last-level cache.
+constexpr int kPairVpt = 8;
+__global__ __launch_bounds__(kBlock) void pair_grad_kernel(const float* logits, float* grad, const RowFactor* factors, int64_t rows, int64_t cols, int runs) {
+    const int64_t row = rows - 1 - (int64_t)(blockIdx.x / (unsigned)runs);
+    const int run = (int)(blockIdx.x % (unsigned)runs);
     const RowFactor f = factors[row];
     const float* x = logits + row * cols;
     float* out = grad + row * cols;
+    const RowShape sh(x, cols);
+    const f4* xv = reinterpret_cast<const f4*>(x + sh.head);
+    f4a4* ov = reinterpret_cast<f4a4*>(out + sh.head);
+    const int first = run * kPairVpt * kBlock + (int)threadIdx.x;
+    const int64_t single = run == 0 ? sh.single((int)threadIdx.x) : -1;
     if (f.target == 0xffffffffu) {
-        for (int64_t c = threadIdx.x; c < cols; c += kBlock) out[c] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kPairVpt; j++)
+            if (first + j * kBlock < sh.n4) ov[first + j * kBlock] = f4{0, 0, 0, 0};
+        if (single >= 0) out[single] = 0.0f;
         return;
     }
-    for (int64_t c = threadIdx.x; c < cols; c += kBlock) {
-        const float v = f.a * exp_of(x[c], f.m, kUnitScale);
-        out[c] = c == (int64_t)f.target ? v - f.c : v;
+    const int tv = (int)f.target - sh.head, t4 = (int)f.target >= sh.head ? tv >> 2 : -1;
+    const f4 off_target = {(tv & 3) == 0 ? f.c : 0.0f, (tv & 3) == 1 ? f.c : 0.0f, (tv & 3) == 2 ? f.c : 0.0f, (tv & 3) == 3 ? f.c : 0.0f};
+    f4 v[kPairVpt];
+#pragma unroll
+    for (int j = 0; j < kPairVpt; j++)
+        if (first + j * kBlock < sh.n4) v[j] = __builtin_nontemporal_load(xv + first + j * kBlock);
+    const float one = single >= 0 ? x[single] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPairVpt; j++) {
+        const int i4 = first + j * kBlock;
+        if (i4 < sh.n4) {
+            f4 r;
+#pragma unroll
+            for (int c = 0; c < 4; c++) r[c] = f.a * exp_of(v[j][c], f.m, kUnitScale);
+            if (i4 == t4) r -= off_target;
+            __builtin_nontemporal_store((f4a4)r, ov + i4);
+        }
+    }
+    if (single >= 0) {
+        const float r = f.a * exp_of(one, f.m, kUnitScale);
+        out[single] = single == (int64_t)f.target ? r - f.c : r;
     }
 }
 
@@ -864,10 +998,7 @@ void seraph_objectives_exchange_spins(int spins) {
     if (spins >= 0) g_spin_limit = spins;
 }
 
-size_t seraph_token_logprobs_ws_bytes(int64_t rows, int64_t cols) {
-    (void)rows; (void)cols;
-    return 0;
-}
+size_t seraph_token_logprobs_ws_bytes(int64_t rows, int64_t cols) { return streamed_ws_bytes(rows, cols); }
 
 int seraph_token_logprobs(const float* logits, const uint32_t* targets, float* logp, float* lse, float* entropy,
                           const uint32_t* seq_starts, int batch, int64_t rows, int64_t cols,
@@ -907,7 +1038,8 @@ int seraph_policy_grad(const float* logits, const uint32_t* actions, const float
 
 size_t seraph_preference_grad_ws_bytes(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    return up16((size_t)rows * sizeof(RowFactor)) + up16((size_t)rows * sizeof(double)) + up16((size_t)rows * sizeof(RowTotals));
+    return up16((size_t)rows * sizeof(RowFactor)) + up16((size_t)rows * sizeof(double)) + up16((size_t)rows * sizeof(RowTotals)) +
+           streamed_ws_bytes(rows, cols);
 }
 
 int seraph_preference_grad(const float* logits, const uint32_t* targets, const float* ref_logp, float* grad,
@@ -929,13 +1061,15 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
     double* logp = reinterpret_cast<double*>(p += up16((size_t)rows * sizeof(RowFactor)));
     RowTotals* totals = reinterpret_cast<RowTotals*>(p += up16((size_t)rows * sizeof(double)));
     PairRowsOp op{{targets, nullptr, seq_starts, 2 * pairs, cols}, totals, logp, factors, logp_rows, kUnitScale};
-    const int rc = launch_rows<PairRowsOp, kNone>(op, logits, nullptr, rows, cols, 0, ws, st);
+    const int rc = launch_rows<PairRowsOp, kNone>(op, logits, nullptr, rows, cols, 0, p + up16((size_t)rows * sizeof(RowTotals)), st);
     if (rc != SERAPH_OK) return rc;
     PreferenceArgs a{ref_logp, loss_pairs, scores, logp_rows, seq_starts, pairs, rows, options->kind, options->average,
                      options->beta, options->label_smoothing, options->margin};
     hipLaunchKernelGGL(pair_kernel, dim3((unsigned)pairs), dim3(kBlock), 0, st, a, totals, logp, factors);
     SERAPH_LAUNCH_CHECK();
-    hipLaunchKernelGGL(pair_grad_kernel, dim3((unsigned)rows), dim3(kBlock), 0, st, logits, grad, factors, cols);
+    const int64_t runs = ceil_div(ceil_div(cols, 4), kPairVpt * kBlock);
+    SERAPH_REQUIRE(rows * runs <= 0x7fffffff, "preference_grad: too many logits: %lld x %lld", (long long)rows, (long long)cols);
+    hipLaunchKernelGGL(pair_grad_kernel, dim3((unsigned)(rows * runs)), dim3(kBlock), 0, st, logits, grad, factors, rows, cols, (int)runs);
     SERAPH_LAUNCH_CHECK();
     return SERAPH_OK;
 }
