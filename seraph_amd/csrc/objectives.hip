@@ -163,72 +163,106 @@ struct DistillOp {
 
 // ---------------------------------------------------------------- a teacher's list
 // Turns a row's list into the mass q of each entry (entries of one id all hold that id's whole mass, added in list order,
-// so whichever of them is used last leaves the same value), its logits z, and the row's sums.  Called by a whole
-// workgroup; the arrays are its LDS.  The logits are gathered before anything of the row is overwritten.
-template <int BLOCK, int K>
+// so whichever of them is used last leaves the same value), its logits z, and the row's sums.  One wave's work: the others
+// of its workgroup go on with the row, and meet the list again behind a barrier.  The logits are gathered before
+// anything of the row is overwritten.
+//
+// Ids listed twice are rare and finding them by comparing all pairs would cost more than all the rest: the ids go into a
+// hash table first, and only where one of them meets itself there are the pairs compared.
+//
+// The list's LDS is sized by the call (list_bytes): with room for the longest list always, short ones would cost the
+// wave of prepare_rows_kernel most of its occupancy.
 struct ListRoom {
-    uint32_t id[K];
-    float q[K], z[K];
-    float red[3][BLOCK / 64];
-    double red64[2][BLOCK / 64];
+    float *q, *z;
+    uint32_t *id, *table;
+    int slots;                                                    // of the table: a power of two, twice the entries at least
 };
+static __host__ __device__ inline int list_slots(int top_k) {
+    int n = 64;
+    while (n < 2 * top_k) n *= 2;
+    return n;
+}
+static size_t list_bytes(int top_k) { return (size_t)(3 * top_k + list_slots(top_k)) * 4; }
+__device__ __forceinline__ ListRoom list_room(void* lds, int top_k) {
+    float* f = reinterpret_cast<float*>(lds);
+    return ListRoom{f, f + top_k, reinterpret_cast<uint32_t*>(f + 2 * top_k), reinterpret_cast<uint32_t*>(f + 3 * top_k), list_slots(top_k)};
+}
+constexpr uint32_t kNoId = 0xffffffffu;
 
-template <int BLOCK, int K>
-__device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, const float* row, int64_t cols, double inv_temp, ExpScale k, ListRoom<BLOCK, K>& room) {
-    const int64_t base = r * l.top_k;
-    float m = kLowest, at = kLowest;
-    for (int i = threadIdx.x; i < l.top_k; i += BLOCK) {
-        const uint32_t id = l.ids[base + i];
+__device__ __forceinline__ void wave_sync() {                     // the wave's own LDS writes are complete and in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, const float* row, int64_t cols, double inv_temp, ExpScale k, const ListRoom& room) {
+    const int lane = (int)threadIdx.x & 63, n = l.top_k;
+    const int64_t base = r * n;
+    float m = kLowest;
+    for (int i = lane; i < n; i += 64) {
+        uint32_t id = l.ids[base + i];
+        if ((int64_t)id >= cols) id = kNoId;
         const float u = l.logit(base + i);
         room.id[i] = id;
         room.q[i] = u;
-        if ((int64_t)id < cols) {
-            const float z = row[id];
-            room.z[i] = z;
-            m = fmaxf(m, u);
-            at = fmaxf(at, z);
+        if (id != kNoId) m = fmaxf(m, u);
+    }
+    for (int i = lane; i < room.slots; i += 64) room.table[i] = kNoId;
+    float at = kLowest;
+    for (int i = lane; i < n; i += 64) {
+        const uint32_t id = room.id[i];
+        const float z = id != kNoId ? row[id] : 0.0f;
+        room.z[i] = z;
+        if (id != kNoId) at = fmaxf(at, z);
+    }
+    wave_sync();
+    bool twice = false;
+    for (int i = lane; i < n; i += 64) {
+        const uint32_t id = room.id[i];
+        if (id == kNoId) continue;
+        for (uint32_t h = (id * 2654435761u) >> 8;; h++) {        // the table is half empty at least: a free slot ends every search
+            const uint32_t found = atomicCAS(&room.table[h & (uint32_t)(room.slots - 1)], kNoId, id);
+            if (found == kNoId) break;
+            if (found == id) { twice = true; break; }
         }
     }
-    m = block_max<BLOCK>(m, room.red[0]);
-    at = block_max<BLOCK>(at, room.red[1]);
+    twice = __any(twice);
+    m = wave_top(m);
+    at = wave_top(at);
     float s = 0.0f;
-    for (int i = threadIdx.x; i < l.top_k; i += BLOCK)
-        if ((int64_t)room.id[i] < cols) s += exp_of(room.q[i], m, k);
-    s = block_sum<BLOCK>(s, room.red[2]);
-    // log q_i = (u_i - m) / T + log_norm
-    const double log_norm = l.lse ? (double)m * inv_temp - (double)l.lse[r] : -log((double)s);
-    const float norm = (float)exp(log_norm);
-    ListSums sums{0.0, 0.0, at};
-    for (int i = threadIdx.x; i < l.top_k; i += BLOCK) {
+    for (int i = lane; i < n; i += 64)
+        if (room.id[i] != kNoId) s += exp_of(room.q[i], m, k);
+    s = wave_total(s);
+    // log q_i = (u_i - m) / T + log_norm; q sums up to s exp(log_norm), which is 1 where the list is the whole distribution
+    const double log_norm = l.lse ? (double)m * inv_temp - (double)l.lse[r] : -log_of(s);
+    const float norm = l.lse ? exp_of((float)log_norm, 0.0f, kUnitScale) : 1.0f / s;
+    double cross = 0.0;
+    for (int i = lane; i < n; i += 64) {
         float p = 0.0f;
-        if ((int64_t)room.id[i] < cols && s != 0.0f) {            // (no entry at all: no mass, not NaN)
+        if (room.id[i] != kNoId && s != 0.0f) {                   // (no entry at all: no mass, not NaN)
             const float u = room.q[i];
             p = exp_of(u, m, k) * norm;
-            if (p != 0.0f)
-                sums.cross += (double)p * (((double)u - (double)m) * inv_temp + log_norm - ((double)room.z[i] - (double)at) * inv_temp);
+            if (p != 0.0f) cross += (double)p * (((double)u - (double)m) * inv_temp + log_norm - ((double)room.z[i] - (double)at) * inv_temp);
         }
-        sums.mass += (double)p;
         room.q[i] = p;
     }
-    sums.mass = block_sum<BLOCK>(sums.mass, room.red64[0]);
-    sums.cross = block_sum<BLOCK>(sums.cross, room.red64[1]);
-    // ids listed twice
-    float part[(K + BLOCK - 1) / BLOCK];
+    cross = wave_total(cross);
+    if (twice) {
+        wave_sync();
+        float part[kMaxTopK / 64];
 #pragma unroll
-    for (int j = 0; j < (K + BLOCK - 1) / BLOCK; j++) {
-        const int i = threadIdx.x + j * BLOCK;
-        part[j] = 0.0f;
-        if (i < l.top_k)
-            for (int o = 0; o < l.top_k; o++) part[j] += room.id[o] == room.id[i] ? room.q[o] : 0.0f;
-    }
-    __syncthreads();
+        for (int j = 0; j < kMaxTopK / 64; j++) {
+            const int i = lane + j * 64;
+            part[j] = 0.0f;
+            if (i < n)
+                for (int o = 0; o < n; o++) part[j] += room.id[o] == room.id[i] ? room.q[o] : 0.0f;
+        }
+        wave_sync();
 #pragma unroll
-    for (int j = 0; j < (K + BLOCK - 1) / BLOCK; j++) {
-        const int i = threadIdx.x + j * BLOCK;
-        if (i < l.top_k) room.q[i] = part[j];
+        for (int j = 0; j < kMaxTopK / 64; j++)
+            if (lane + j * 64 < n) room.q[lane + j * 64] = part[j];
     }
-    __syncthreads();
-    return sums;
+    wave_sync();
+    return ListSums{s == 0.0f ? 0.0 : l.lse ? (double)s * (double)norm : s == s ? 1.0 : (double)s, cross, at};
 }
 
 // ---------------------------------------------------------------- rows held in registers
@@ -238,7 +272,7 @@ template <class Op, int EXTRA, int VPT>
 __global__ __launch_bounds__(kBlock) void held_rows_kernel(Op op, const float* logits, float* grad, int cols) {
     __shared__ float red[3][kBlock / 64];
     __shared__ RowGrad bcast;
-    __shared__ ListRoom<kBlock, Op::kList ? kMaxTopK : 1> room;
+    extern __shared__ char list_lds[];
     const int64_t row = blockIdx.x;
     const float* x = logits + row * cols;
     float* out = Op::kGrad ? grad + row * cols : nullptr;
@@ -264,8 +298,12 @@ __global__ __launch_bounds__(kBlock) void held_rows_kernel(Op op, const float* l
         const int64_t t = op.target(row);
         if (t >= 0) zt = x[t];
     }
+    ListRoom room{};
     ListSums sums{0.0, 0.0, 0.0f};
-    if constexpr (Op::kList) sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+    if constexpr (Op::kList) {
+        room = list_room(list_lds, op.list.top_k);
+        if (threadIdx.x < 64) sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+    }
     const ExpScale ks = op.k;
     float m = fmaxf(kLowest, one);
 #pragma unroll
@@ -316,7 +354,7 @@ __global__ __launch_bounds__(kBlock) void held_rows_kernel(Op op, const float* l
             __syncthreads();
             for (int i = threadIdx.x; i < op.list.top_k; i += kBlock) {
                 const uint32_t id = room.id[i];
-                if ((int64_t)id < cols) out[id] = grad_at<EXTRA>(room.z[i], m, ks, g) - es * room.q[i] - ((int64_t)id == g.target ? g.c : 0.0f);
+                if (id != kNoId) out[id] = grad_at<EXTRA>(room.z[i], m, ks, g) - es * room.q[i] - ((int64_t)id == g.target ? g.c : 0.0f);
             }
         }
     }
@@ -373,35 +411,37 @@ __device__ __forceinline__ RowStats against(RowStats st, float m, ExpScale k) {
     return o;
 }
 
-// Clears the row's records and gathers its target's logit; one lane per row, or (rows with lists) one workgroup per row.
+// Clears the rows' records and gathers what belongs to a row as a whole.  A wave takes kPrepRows rows, a lane each, or, of an
+// op with lists, one row.
+constexpr int kPrepRows = 16;
 template <class Op>
-__global__ __launch_bounds__(kBlock) void prepare_rows_kernel(Op op, const float* logits, int64_t rows, int64_t cols, int P, RowPrep* prep,
-                                                              PartRecord* records, float* list_q, float* list_z) {
+__global__ __launch_bounds__(64) void prepare_rows_kernel(Op op, const float* logits, int64_t rows, int64_t cols, int P, RowPrep* prep,
+                                                          PartRecord* records, float* list_q, float* list_z) {
+    constexpr int kTake = Op::kList ? 1 : kPrepRows;
+    const int64_t first = (int64_t)blockIdx.x * kTake;
+    const int here = rows - first < kTake ? (int)(rows - first) : kTake;
+    unsigned long long* words = reinterpret_cast<unsigned long long*>(records + first * P);
+    for (int i = threadIdx.x; i < here * P * 4; i += 64) __hip_atomic_store(words + i, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if constexpr (Op::kList) {
-        __shared__ ListRoom<kBlock, kMaxTopK> room;
-        const int64_t row = blockIdx.x;
-        unsigned long long* words = reinterpret_cast<unsigned long long*>(records + row * P);
-        for (int i = threadIdx.x; i < P * 4; i += kBlock) __hip_atomic_store(words + i, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        extern __shared__ char list_lds[];
+        const ListRoom room = list_room(list_lds, op.list.top_k);
+        ListSums sums{0.0, 0.0, 0.0f};
+        const int64_t row = first;
         const float* x = logits + row * cols;
         const bool live = op.live(row);
-        RowPrep p{{0.0, 0.0, 0.0f}, 0.0f, live ? 1 : 0};
         if (live) {
-            p.sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
-            for (int i = threadIdx.x; i < op.list.top_k; i += kBlock) {
+            sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+            for (int i = threadIdx.x; i < op.list.top_k; i += 64) {
                 list_q[row * op.list.top_k + i] = room.q[i];
                 list_z[row * op.list.top_k + i] = room.z[i];
             }
         }
         if (threadIdx.x == 0) {
             const int64_t t = live ? op.target(row) : -1;
-            if (t >= 0) p.zt = x[t];
-            prep[row] = p;
+            prep[row] = RowPrep{sums, t >= 0 ? x[t] : 0.0f, live ? 1 : 0};
         }
-    } else {
-        const int64_t row = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-        if (row >= rows) return;
-        unsigned long long* words = reinterpret_cast<unsigned long long*>(records + row * P);
-        for (int i = 0; i < P * 4; i++) __hip_atomic_store(words + i, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else if ((int)threadIdx.x < here) {
+        const int64_t row = first + threadIdx.x;
         const bool live = op.live(row);
         const int64_t t = live ? op.target(row) : -1;
         prep[row] = RowPrep{{0.0, 0.0, 0.0f}, t >= 0 ? logits[row * cols + t] : 0.0f, live ? 1 : 0};
@@ -537,9 +577,9 @@ __global__ __launch_bounds__(kBlock, kPartsPerCu) void shared_rows_kernel(Op op,
                 if (todo) {
                     if (lane < P) parts[lane] = got;
                 } else {
-                    const float rm = wave_max(got.m);
+                    const float rm = wave_top(got.m);
                     const RowStats o = against<EXTRA>(got, rm, ks);
-                    const RowStats total{rm, wave_sum(o.s), EXTRA != kNone ? wave_sum(o.x) : 0.0f};
+                    const RowStats total{rm, wave_total(o.s), EXTRA != kNone ? wave_total(o.x) : 0.0f};
                     if (lane == 0) {
                         bcast.st = total;
                         bcast.g = op.template finish<EXTRA>(row, total, prep[row].zt, prep[row].sums, part == 0);
@@ -646,8 +686,9 @@ static int launch_shared(const Op& op, const float* logits, float* grad, int64_t
     PartRecord* records = reinterpret_cast<PartRecord*>(p += up16((size_t)rows * sizeof(RowPrep)));
     float* list_q = reinterpret_cast<float*>(p += (size_t)rows * P * sizeof(PartRecord));
     float* list_z = reinterpret_cast<float*>(p += up16((size_t)rows * (size_t)top_k * 4));
-    const unsigned prep_grid = Op::kList ? (unsigned)rows : (unsigned)ceil_div(rows, kBlock);
-    hipLaunchKernelGGL((prepare_rows_kernel<Op>), dim3(prep_grid), dim3(kBlock), 0, st, op, logits, rows, cols, P, prep, records, list_q, list_z);
+    const size_t lds = Op::kList ? list_bytes((int)top_k) : 0;
+    const unsigned prep_grid = (unsigned)(Op::kList ? rows : ceil_div(rows, kPrepRows));
+    hipLaunchKernelGGL((prepare_rows_kernel<Op>), dim3(prep_grid), dim3(64), lds, st, op, logits, rows, cols, P, prep, records, list_q, list_z);
     SERAPH_LAUNCH_CHECK();
     int64_t G = (int64_t)num_compute_units() * kPartsPerCu / P * P;
     if (G < P) G = P;
@@ -732,9 +773,9 @@ __global__ __launch_bounds__(kBlock) void join_runs_kernel(Op op, const float* l
         return;
     }
     const RowStats got = lane < splits ? runs[row * splits + lane] : RowStats{kLowest, 0.0f, 0.0f};
-    const float m = wave_max(got.m);
+    const float m = wave_top(got.m);
     const RowStats o = against<EXTRA>(got, m, op.k);
-    const RowStats total{m, wave_sum(o.s), EXTRA != kNone ? wave_sum(o.x) : 0.0f};
+    const RowStats total{m, wave_total(o.s), EXTRA != kNone ? wave_total(o.x) : 0.0f};
     if (lane == 0) op.template finish<EXTRA>(row, total, logits[row * cols + op.target(row)], ListSums{0.0, 0.0, 0.0f});
 }
 
@@ -767,7 +808,7 @@ template <class Op, int EXTRA>
 __global__ __launch_bounds__(kBlock) void swept_rows_kernel(Op op, const float* logits, float* grad, int64_t cols) {
     __shared__ float red[3][kBlock / 64];
     __shared__ RowGrad bcast;
-    __shared__ ListRoom<kBlock, Op::kList ? kMaxTopK : 1> room;
+    extern __shared__ char list_lds[];
     const int64_t row = blockIdx.x;
     float* out = grad + row * cols;
     if (!op.live(row)) {
@@ -789,8 +830,12 @@ __global__ __launch_bounds__(kBlock) void swept_rows_kernel(Op op, const float* 
     }
     st.s = block_sum<kBlock>(s, red[1]);
     st.x = EXTRA == kNone ? 0.0f : block_sum<kBlock>(ex, red[2]);
+    ListRoom room{};
     ListSums sums{0.0, 0.0, 0.0f};
-    if constexpr (Op::kList) sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+    if constexpr (Op::kList) {
+        room = list_room(list_lds, op.list.top_k);
+        if (threadIdx.x < 64) sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+    }
     if (threadIdx.x == 0) {
         const int64_t t = op.target(row);
         bcast = op.template finish<EXTRA>(row, st, t >= 0 ? x[t] : 0.0f, sums);
@@ -806,16 +851,17 @@ __global__ __launch_bounds__(kBlock) void swept_rows_kernel(Op op, const float* 
         __syncthreads();                                          // the sweep has written every entry's place
         for (int i = threadIdx.x; i < op.list.top_k; i += kBlock) {
             const uint32_t id = room.id[i];
-            if ((int64_t)id < cols) out[id] = grad_at<EXTRA>(room.z[i], st.m, k, g) - es * room.q[i] - ((int64_t)id == g.target ? g.c : 0.0f);
+            if (id != kNoId) out[id] = grad_at<EXTRA>(room.z[i], st.m, k, g) - es * room.q[i] - ((int64_t)id == g.target ? g.c : 0.0f);
         }
     }
 }
 
 template <class Op, int EXTRA>
 static int launch_rows(const Op& op, const float* logits, float* grad, int64_t rows, int64_t cols, int64_t top_k, void* ws, hipStream_t st) {
+    const size_t lds = Op::kList ? list_bytes((int)top_k) : 0;
     if (cols <= 32768) {
         const int64_t n4 = cols / 4;
-#define HELD(V) hipLaunchKernelGGL((held_rows_kernel<Op, EXTRA, V>), dim3((unsigned)rows), dim3(kBlock), 0, st, op, logits, grad, (int)cols)
+#define HELD(V) hipLaunchKernelGGL((held_rows_kernel<Op, EXTRA, V>), dim3((unsigned)rows), dim3(kBlock), lds, st, op, logits, grad, (int)cols)
         if (n4 <= 1 * kBlock) HELD(1);
         else if (n4 <= 2 * kBlock) HELD(2);
         else if (n4 <= 4 * kBlock) HELD(4);
@@ -828,7 +874,7 @@ static int launch_rows(const Op& op, const float* logits, float* grad, int64_t r
     }
     if constexpr (Op::kGrad) {
         if (is_shared(cols)) return launch_shared<Op, EXTRA>(op, logits, grad, rows, cols, top_k, ws, st);
-        hipLaunchKernelGGL((swept_rows_kernel<Op, EXTRA>), dim3((unsigned)rows), dim3(kBlock), 0, st, op, logits, grad, cols);
+        hipLaunchKernelGGL((swept_rows_kernel<Op, EXTRA>), dim3((unsigned)rows), dim3(kBlock), lds, st, op, logits, grad, cols);
         SERAPH_LAUNCH_CHECK();
         return SERAPH_OK;
     } else {

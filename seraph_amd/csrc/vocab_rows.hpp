@@ -76,9 +76,50 @@ __device__ __forceinline__ float extra_of(float z, float m, float e) {
     return 0.0f;
 }
 
+// Reductions over a wave by data-parallel moves: lanes 1, 2, 4 and 8 below within each row of 16, then the rows' last
+// lanes into the next rows; lane 63 ends with the whole and hands it to all as a scalar.  Six dependent additions, where
+// shuffles through the LDS crossbar put some 60 cycles behind each.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float v, float otherwise) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, otherwise), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v, double otherwise) {
+    const uint64_t a = __builtin_bit_cast(uint64_t, v), b = __builtin_bit_cast(uint64_t, otherwise);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)b, (int)(uint32_t)a, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)(b >> 32), (int)(uint32_t)(a >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ float last_lane(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63)); }
+__device__ __forceinline__ double last_lane(double v) {
+    const uint64_t a = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)a, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(a >> 32), 63);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+enum { kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143 };
+template <class T>
+__device__ __forceinline__ T wave_total(T v) {                    // every lane of the wave is active
+    v += moved<kShr1, 0xf>(v, (T)0);
+    v += moved<kShr2, 0xf>(v, (T)0);
+    v += moved<kShr4, 0xf>(v, (T)0);
+    v += moved<kShr8, 0xf>(v, (T)0);
+    v += moved<kBcast15, 0xa>(v, (T)0);
+    v += moved<kBcast31, 0xc>(v, (T)0);
+    return last_lane(v);
+}
+__device__ __forceinline__ float wave_top(float v) {
+    v = fmaxf(v, moved<kShr1, 0xf>(v, v));
+    v = fmaxf(v, moved<kShr2, 0xf>(v, v));
+    v = fmaxf(v, moved<kShr4, 0xf>(v, v));
+    v = fmaxf(v, moved<kShr8, 0xf>(v, v));
+    v = fmaxf(v, moved<kBcast15, 0xa>(v, v));
+    v = fmaxf(v, moved<kBcast31, 0xc>(v, v));
+    return last_lane(v);
+}
+
 template <int BLOCK>
 __device__ __forceinline__ float block_max(float v, float* lds) {
-    v = wave_max(v);
+    v = wave_top(v);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     float r = lds[0];
@@ -88,7 +129,7 @@ __device__ __forceinline__ float block_max(float v, float* lds) {
 }
 template <int BLOCK, class T>
 __device__ __forceinline__ T block_sum(T v, T* lds) {
-    v = wave_sum(v);
+    v = wave_total(v);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     T r = lds[0];
@@ -96,12 +137,11 @@ __device__ __forceinline__ T block_sum(T v, T* lds) {
     for (int w = 1; w < BLOCK / 64; w++) r += lds[w];
     return r;
 }
-
 // both sums over the workgroup behind one barrier; lds holds 2 BLOCK / 64 floats
 template <int BLOCK>
 __device__ __forceinline__ void block_sum2(float& a, float& b, float* lds) {
-    a = wave_sum(a);
-    b = wave_sum(b);
+    a = wave_total(a);
+    b = wave_total(b);
     if ((threadIdx.x & 63) == 0) {
         lds[threadIdx.x >> 6] = a;
         lds[BLOCK / 64 + (threadIdx.x >> 6)] = b;

@@ -130,7 +130,8 @@ def _ptr(t):
 
 
 class _on:
-    """Makes `device` the current one for a call, where it is not."""
+    """Makes `device` the current one for a call, where it is not, and gives the handle of its current stream (without
+    the stream object around it, whose construction takes as long as a launch)."""
 
     def __init__(self, device):
         self.device, self.before = device.index, None
@@ -140,7 +141,7 @@ class _on:
         if now != self.device:
             self.before = now
             torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device)
 
     def __exit__(self, *exc):
         if self.before is not None:
