@@ -162,68 +162,92 @@ struct DistillOp {
 };
 
 // ---------------------------------------------------------------- a teacher's list
-// Turns a row's list into the mass q of each entry (entries of one id all hold that id's whole mass, added in list order,
-// so whichever of them is used last leaves the same value), its logits z, and the row's sums.  One wave's work: the others
-// of its workgroup go on with the row, and meet the list again behind a barrier.  The logits are gathered before
-// anything of the row is overwritten.
+// Turns a row's list into the mass q of each entry, its logits z, and the row's sums.  One wave's work: the others of its
+// workgroup go on with the row, and meet the list again behind a barrier.  The logits are gathered before anything of
+// the row is overwritten.
 //
-// Ids listed twice are rare and finding them by comparing all pairs would cost more than all the rest: the ids go into a
-// hash table first, and only where one of them meets itself there are the pairs compared.
+// The entries are chained in buckets.  Where the workgroup holds the whole row (HELD) a bucket is a vector of it, so the
+// lane that is about to store a vector finds the entries in it by one look; elsewhere it is a hash of the id.  Either
+// way an id listed twice meets itself in its chain.  That is rare, and only then are all pairs compared: each entry of such an
+// id takes the id's whole mass, added in list order (HELD: the first does and the others take none, so that the
+// order of a chain, which is the order of atomics, changes nothing).
 //
-// The list's LDS is sized by the call (list_bytes): with room for the longest list always, short ones would cost the
-// wave of prepare_rows_kernel most of its occupancy.
+// The list's LDS is sized by the call: with room for the longest list always, short ones would cost the wave of
+// prepare_rows_kernel most of its occupancy.
 struct ListRoom {
     float *q, *z;
-    uint32_t *id, *table;
-    int slots;                                                    // of the table: a power of two, twice the entries at least
+    uint32_t *id, *next, *first;                                  // next, first: an entry's number plus 1, or 0
+    int buckets;
 };
-static __host__ __device__ inline int list_slots(int top_k) {
+static __host__ __device__ inline int hash_buckets(int top_k) {
     int n = 64;
-    while (n < 2 * top_k) n *= 2;
+    while (n < top_k) n *= 2;
     return n;
 }
-static size_t list_bytes(int top_k) { return (size_t)(3 * top_k + list_slots(top_k)) * 4; }
-__device__ __forceinline__ ListRoom list_room(void* lds, int top_k) {
+static size_t list_bytes(int top_k, int buckets) { return (size_t)(4 * top_k + buckets) * 4; }
+__device__ __forceinline__ ListRoom list_room(void* lds, int top_k, int buckets) {
     float* f = reinterpret_cast<float*>(lds);
-    return ListRoom{f, f + top_k, reinterpret_cast<uint32_t*>(f + 2 * top_k), reinterpret_cast<uint32_t*>(f + 3 * top_k), list_slots(top_k)};
+    uint32_t* u = reinterpret_cast<uint32_t*>(f + 2 * top_k);
+    return ListRoom{f, f + top_k, u, u + top_k, u + 2 * top_k, buckets};
 }
 constexpr uint32_t kNoId = 0xffffffffu;
+
+// HELD: 0 the single values ahead of the vectors, 1 + i vector i, 1 + n4 those behind
+template <bool HELD>
+__device__ __forceinline__ int list_bucket(const ListRoom& room, const RowShape& sh, uint32_t id) {
+    if (!HELD) return (int)((id * 2654435761u) >> 8 & (uint32_t)(room.buckets - 1));
+    const int i4 = ((int)id - sh.head) >> 2;
+    return (int)id < sh.head ? 0 : i4 < sh.n4 ? 1 + i4 : 1 + sh.n4;
+}
 
 __device__ __forceinline__ void wave_sync() {                     // the wave's own LDS writes are complete and in order
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
 
-__device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, const float* row, int64_t cols, double inv_temp, ExpScale k, const ListRoom& room) {
+template <bool HELD>
+__device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, const float* row, const RowShape& sh, int64_t cols, double inv_temp, ExpScale k,
+                                              const ListRoom& room) {
     const int lane = (int)threadIdx.x & 63, n = l.top_k;
     const int64_t base = r * n;
-    float m = kLowest;
-    for (int i = lane; i < n; i += 64) {
-        uint32_t id = l.ids[base + i];
-        if ((int64_t)id >= cols) id = kNoId;
-        const float u = l.logit(base + i);
-        room.id[i] = id;
-        room.q[i] = u;
-        if (id != kNoId) m = fmaxf(m, u);
-    }
-    for (int i = lane; i < room.slots; i += 64) room.table[i] = kNoId;
-    float at = kLowest;
-    for (int i = lane; i < n; i += 64) {
-        const uint32_t id = room.id[i];
-        const float z = id != kNoId ? row[id] : 0.0f;
-        room.z[i] = z;
-        if (id != kNoId) at = fmaxf(at, z);
+    float m = kLowest, at = kLowest;
+    for (int i = lane; i < room.buckets; i += 64) room.first[i] = 0u;
+    wave_sync();
+    constexpr int kAhead = 4;                                     // entries in flight per lane: a list of 256 waits for memory twice
+    for (int i0 = lane; i0 < n; i0 += 64 * kAhead) {
+        uint32_t id[kAhead];
+        float u[kAhead], z[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int i = i0 + j * 64;
+            id[j] = i < n ? l.ids[base + i] : kNoId;
+            u[j] = i < n ? l.logit(base + i) : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            if ((int64_t)id[j] >= cols) id[j] = kNoId;
+            z[j] = id[j] != kNoId ? row[id[j]] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int i = i0 + j * 64;
+            if (i >= n) break;
+            room.id[i] = id[j];
+            room.q[i] = u[j];
+            room.z[i] = z[j];
+            if (id[j] != kNoId) {
+                room.next[i] = atomicExch(&room.first[list_bucket<HELD>(room, sh, id[j])], (uint32_t)i + 1u);
+                m = fmaxf(m, u[j]);
+                at = fmaxf(at, z[j]);
+            }
+        }
     }
     wave_sync();
     bool twice = false;
     for (int i = lane; i < n; i += 64) {
         const uint32_t id = room.id[i];
         if (id == kNoId) continue;
-        for (uint32_t h = (id * 2654435761u) >> 8;; h++) {        // the table is half empty at least: a free slot ends every search
-            const uint32_t found = atomicCAS(&room.table[h & (uint32_t)(room.slots - 1)], kNoId, id);
-            if (found == kNoId) break;
-            if (found == id) { twice = true; break; }
-        }
+        for (uint32_t o = room.first[list_bucket<HELD>(room, sh, id)]; o; o = room.next[o - 1]) twice |= o != (uint32_t)i + 1u && room.id[o - 1] == id;
     }
     twice = __any(twice);
     m = wave_top(m);
@@ -253,8 +277,15 @@ __device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, c
         for (int j = 0; j < kMaxTopK / 64; j++) {
             const int i = lane + j * 64;
             part[j] = 0.0f;
-            if (i < n)
-                for (int o = 0; o < n; o++) part[j] += room.id[o] == room.id[i] ? room.q[o] : 0.0f;
+            if (i < n) {
+                bool earlier = false;
+                for (int o = 0; o < n; o++)
+                    if (room.id[o] == room.id[i]) {
+                        part[j] += room.q[o];
+                        earlier |= o < i;
+                    }
+                if (HELD && earlier) part[j] = 0.0f;
+            }
         }
         wave_sync();
 #pragma unroll
@@ -268,9 +299,12 @@ __device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, c
 // ---------------------------------------------------------------- rows held in registers
 // One workgroup owns a row of up to 4 kBlock VPT columns (and seven single values) and holds it in its registers: a logit
 // crosses memory once in each direction.
-template <class Op, int EXTRA, int VPT>
-__global__ __launch_bounds__(kBlock) void held_rows_kernel(Op op, const float* logits, float* grad, int cols) {
-    __shared__ float red[3][kBlock / 64];
+// Waves per SIMD asked for: at eight, all of 2048 rows of 8192 columns are on the chip at once (21.4 us; at six 24.7 us); the
+// list ops would spill.
+constexpr int held_waves(int vpt, bool list) { return list ? 4 : vpt <= 8 ? 8 : vpt <= 12 ? 5 : 4; }
+template <class Op, int EXTRA, int BLOCK, int VPT>
+__global__ __launch_bounds__(BLOCK, held_waves(VPT, Op::kList)) void held_rows_kernel(Op op, const float* logits, float* grad, int cols) {
+    __shared__ float red[3][BLOCK / 64];
     __shared__ RowGrad bcast;
     extern __shared__ char list_lds[];
     const int64_t row = blockIdx.x;
@@ -283,7 +317,7 @@ __global__ __launch_bounds__(kBlock) void held_rows_kernel(Op op, const float* l
         if constexpr (Op::kGrad) {
             const SlotBuffer gs(out + sh.head, sh.n4);
 #pragma unroll
-            for (int k = 0; k < VPT; k++) gs.store<kNontemporal>(f4{0, 0, 0, 0}, (k * kBlock + (int)threadIdx.x) * 16);
+            for (int k = 0; k < VPT; k++) gs.store<kNontemporal>(f4{0, 0, 0, 0}, (k * BLOCK + (int)threadIdx.x) * 16);
             if (single >= 0) out[single] = 0.0f;
         }
         if (threadIdx.x == 0) op.dead(row);
@@ -291,7 +325,7 @@ __global__ __launch_bounds__(kBlock) void held_rows_kernel(Op op, const float* l
     }
     f4 v[VPT];
 #pragma unroll
-    for (int k = 0; k < VPT; k++) v[k] = xs.load<kNontemporal>((k * kBlock + (int)threadIdx.x) * 16);
+    for (int k = 0; k < VPT; k++) v[k] = xs.load<kNontemporal>((k * BLOCK + (int)threadIdx.x) * 16);
     float one = single >= 0 ? x[single] : -INFINITY;
     float zt = 0.0f;
     if (threadIdx.x == 0) {
@@ -301,17 +335,17 @@ __global__ __launch_bounds__(kBlock) void held_rows_kernel(Op op, const float* l
     ListRoom room{};
     ListSums sums{0.0, 0.0, 0.0f};
     if constexpr (Op::kList) {
-        room = list_room(list_lds, op.list.top_k);
-        if (threadIdx.x < 64) sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+        room = list_room(list_lds, op.list.top_k, sh.n4 + 2);
+        if (threadIdx.x < 64) sums = read_list<true>(op.list, row, x, sh, cols, op.inv_temp, op.k, room);
     }
     const ExpScale ks = op.k;
     float m = fmaxf(kLowest, one);
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
-        if (k * kBlock + (int)threadIdx.x >= sh.n4) v[k] = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (k * BLOCK + (int)threadIdx.x >= sh.n4) v[k] = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
     }
-    m = block_max<kBlock>(m, red[0]);
+    m = block_max<BLOCK>(m, red[0]);
     float e1 = exp_of(one, m, ks), s = e1, ex = EXTRA != kNone ? extra_of<EXTRA>(one, m, e1) : 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
@@ -322,40 +356,44 @@ __global__ __launch_bounds__(kBlock) void held_rows_kernel(Op op, const float* l
             if (EXTRA != kNone) ex += extra_of<EXTRA>(v[k][c], m, e);
             else if (Op::kGrad) v[k][c] = e;                      // the gradient is a multiple of it
         }
+        if (!Op::kList) asm volatile("" : "+v"(v[k]));            // four values stay the four registers that a store takes
     }
-    if (EXTRA != kNone) block_sum2<kBlock>(s, ex, red[1]);
-    else s = block_sum<kBlock>(s, red[1]);
+    if (EXTRA != kNone) block_sum2<BLOCK>(s, ex, red[1]);
+    else s = block_sum<BLOCK>(s, red[1]);
     if (threadIdx.x == 0) bcast = op.template finish<EXTRA>(row, RowStats{m, s, ex}, zt, sums);
     if constexpr (Op::kGrad) {
         __syncthreads();
         const RowGrad g = bcast;
         const SlotBuffer gs(out + sh.head, sh.n4);
+        float es = 0.0f;
+        if constexpr (Op::kList) es = op.entry_scale(row);
         const int tv = (int)g.target - sh.head, t4 = g.target >= sh.head ? tv >> 2 : -1;      // the target's place among the vectors
         const f4 off_target = {(tv & 3) == 0 ? g.c : 0.0f, (tv & 3) == 1 ? g.c : 0.0f, (tv & 3) == 2 ? g.c : 0.0f, (tv & 3) == 3 ? g.c : 0.0f};
         // the exponentials are formed again from the logits: kept from the sums they would double the registers of a row
         if (EXTRA != kNone) asm volatile("" : "+v"(m));
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
-            const int i4 = k * kBlock + (int)threadIdx.x;
+            const int i4 = k * BLOCK + (int)threadIdx.x;
             f4 r;
 #pragma unroll
             for (int c = 0; c < 4; c++) r[c] = EXTRA == kNone ? g.a * v[k][c] : grad_at<EXTRA>(v[k][c], m, ks, g);
             if (t4 == i4) r -= off_target;
+            if constexpr (Op::kList) {
+                for (uint32_t o = i4 < sh.n4 ? room.first[1 + i4] : 0u; o; o = room.next[o - 1]) {
+                    const int c = ((int)room.id[o - 1] - sh.head) & 3;
+                    const float q = es * room.q[o - 1];
+                    r -= f4{c == 0 ? q : 0.0f, c == 1 ? q : 0.0f, c == 2 ? q : 0.0f, c == 3 ? q : 0.0f};
+                }
+            }
             gs.store<kNontemporal>(r, i4 * 16);
         }
         if (single >= 0) {
-            const float r = grad_at<EXTRA>(one, m, ks, g);
-            out[single] = single == g.target ? r - g.c : r;
-        }
-        if constexpr (Op::kList) {
-            const float es = op.entry_scale(row);
-            // the entries' places have been written by other lanes, and those stores are complete before the second ones
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            for (int i = threadIdx.x; i < op.list.top_k; i += kBlock) {
-                const uint32_t id = room.id[i];
-                if (id != kNoId) out[id] = grad_at<EXTRA>(room.z[i], m, ks, g) - es * room.q[i] - ((int64_t)id == g.target ? g.c : 0.0f);
-            }
+            float r = grad_at<EXTRA>(one, m, ks, g);
+            if (single == g.target) r -= g.c;
+            if constexpr (Op::kList)
+                for (uint32_t o = room.first[single < sh.head ? 0 : 1 + sh.n4]; o; o = room.next[o - 1])
+                    if (room.id[o - 1] == (uint32_t)single) r -= es * room.q[o - 1];
+            out[single] = r;
         }
     }
 }
@@ -424,13 +462,13 @@ __global__ __launch_bounds__(64) void prepare_rows_kernel(Op op, const float* lo
     for (int i = threadIdx.x; i < here * P * 4; i += 64) __hip_atomic_store(words + i, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if constexpr (Op::kList) {
         extern __shared__ char list_lds[];
-        const ListRoom room = list_room(list_lds, op.list.top_k);
+        const ListRoom room = list_room(list_lds, op.list.top_k, hash_buckets(op.list.top_k));
         ListSums sums{0.0, 0.0, 0.0f};
         const int64_t row = first;
         const float* x = logits + row * cols;
         const bool live = op.live(row);
         if (live) {
-            sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+            sums = read_list<false>(op.list, row, x, RowShape(x, cols), cols, op.inv_temp, op.k, room);
             for (int i = threadIdx.x; i < op.list.top_k; i += 64) {
                 list_q[row * op.list.top_k + i] = room.q[i];
                 list_z[row * op.list.top_k + i] = room.z[i];
@@ -686,7 +724,7 @@ static int launch_shared(const Op& op, const float* logits, float* grad, int64_t
     PartRecord* records = reinterpret_cast<PartRecord*>(p += up16((size_t)rows * sizeof(RowPrep)));
     float* list_q = reinterpret_cast<float*>(p += (size_t)rows * P * sizeof(PartRecord));
     float* list_z = reinterpret_cast<float*>(p += up16((size_t)rows * (size_t)top_k * 4));
-    const size_t lds = Op::kList ? list_bytes((int)top_k) : 0;
+    const size_t lds = Op::kList ? list_bytes((int)top_k, hash_buckets((int)top_k)) : 0;
     const unsigned prep_grid = (unsigned)(Op::kList ? rows : ceil_div(rows, kPrepRows));
     hipLaunchKernelGGL((prepare_rows_kernel<Op>), dim3(prep_grid), dim3(64), lds, st, op, logits, rows, cols, P, prep, records, list_q, list_z);
     SERAPH_LAUNCH_CHECK();
@@ -833,8 +871,8 @@ __global__ __launch_bounds__(kBlock) void swept_rows_kernel(Op op, const float* 
     ListRoom room{};
     ListSums sums{0.0, 0.0, 0.0f};
     if constexpr (Op::kList) {
-        room = list_room(list_lds, op.list.top_k);
-        if (threadIdx.x < 64) sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
+        room = list_room(list_lds, op.list.top_k, hash_buckets(op.list.top_k));
+        if (threadIdx.x < 64) sums = read_list<false>(op.list, row, x, RowShape(x, cols), cols, op.inv_temp, op.k, room);
     }
     if (threadIdx.x == 0) {
         const int64_t t = op.target(row);
@@ -858,16 +896,18 @@ __global__ __launch_bounds__(kBlock) void swept_rows_kernel(Op op, const float* 
 
 template <class Op, int EXTRA>
 static int launch_rows(const Op& op, const float* logits, float* grad, int64_t rows, int64_t cols, int64_t top_k, void* ws, hipStream_t st) {
-    const size_t lds = Op::kList ? list_bytes((int)top_k) : 0;
+    const size_t lds = Op::kList ? list_bytes((int)top_k, cols <= 32768 ? (int)cols / 4 + 2 : hash_buckets((int)top_k)) : 0;
     if (cols <= 32768) {
         const int64_t n4 = cols / 4;
-#define HELD(V) hipLaunchKernelGGL((held_rows_kernel<Op, EXTRA, V>), dim3((unsigned)rows), dim3(kBlock), lds, st, op, logits, grad, (int)cols)
-        if (n4 <= 1 * kBlock) HELD(1);
-        else if (n4 <= 2 * kBlock) HELD(2);
-        else if (n4 <= 4 * kBlock) HELD(4);
-        else if (n4 <= 8 * kBlock) HELD(8);
-        else if (n4 <= 16 * kBlock) HELD(16);
-        else HELD(32);
+#define HELD(B, V) hipLaunchKernelGGL((held_rows_kernel<Op, EXTRA, B, V>), dim3((unsigned)rows), dim3(B), lds, st, op, logits, grad, (int)cols)
+        if (n4 <= 256) HELD(256, 1);
+        else if (n4 <= 2 * 256) HELD(256, 2);
+        else if (n4 <= 4 * 256) HELD(256, 4);
+        else if (n4 <= 8 * 256) HELD(256, 8);
+        else if (n4 <= 12 * 256) HELD(256, 12);
+        else if (n4 <= 8 * 512) HELD(512, 8);
+        else if (n4 <= 12 * 512) HELD(512, 12);
+        else HELD(512, 16);
 #undef HELD
         SERAPH_LAUNCH_CHECK();
         return SERAPH_OK;
