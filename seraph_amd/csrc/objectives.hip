@@ -740,7 +740,8 @@ static int launch_shared(const Op& op, const float* logits, float* grad, int64_t
 // ---------------------------------------------------------------- long rows read once
 // Forward only: nothing has to be held.  A row is cut into `splits` runs of vectors, each streamed by one workgroup that keeps
 // a running maximum and sums per lane; one wave per row then puts the runs' results together.  Splitting serves
-// few rows, which alone would leave most of the chip idle, and evens out the last round of many.
+// few rows, which alone would leave most of the chip idle, and evens out the last round of many.  A row in one run (runs
+// NULL) is finished by its own workgroup.
 template <int EXTRA>
 __device__ __forceinline__ void add_logit(RowStats& st, float z, ExpScale k) {
     const float e = exp_of(z, st.m, k);
@@ -748,17 +749,22 @@ __device__ __forceinline__ void add_logit(RowStats& st, float z, ExpScale k) {
     if (EXTRA != kNone) st.x += extra_of<EXTRA>(z, st.m, e);
 }
 
-template <class Op, int EXTRA>
-__global__ __launch_bounds__(kBlock) void streamed_rows_kernel(Op op, const float* logits, int64_t cols, int splits, RowStats* runs) {
+template <class Op, int EXTRA, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void streamed_rows_kernel(Op op, const float* logits, int64_t cols, int splits, RowStats* runs) {
     constexpr int kAhead = 8;                                     // vectors in flight per lane
-    __shared__ float red[3][kBlock / 64];
+    __shared__ float red[3][BLOCK / 64];
     const int64_t row = blockIdx.x / (unsigned)splits;
     const int run = (int)(blockIdx.x % (unsigned)splits);
-    if (!op.live(row)) return;
+    if (!op.live(row)) {
+        if (run == 0 && threadIdx.x == 0) op.dead(row);
+        return;
+    }
+    float zt = 0.0f;
+    if (!runs && threadIdx.x == 0) zt = logits[row * cols + op.target(row)];
     const float* x = logits + row * cols;
     const RowShape sh(x, cols);
     const f4* xv = reinterpret_cast<const f4*>(x + sh.head);
-    const int per_run = ((sh.n4 + splits - 1) / splits + kBlock - 1) / kBlock * kBlock;
+    const int per_run = ((sh.n4 + splits - 1) / splits + BLOCK - 1) / BLOCK * BLOCK;
     const int first = run * per_run, end = first + per_run < sh.n4 ? first + per_run : sh.n4;
     const ExpScale ks = op.k;
     RowStats st{kLowest, 0.0f, 0.0f};
@@ -768,11 +774,7 @@ __global__ __launch_bounds__(kBlock) void streamed_rows_kernel(Op op, const floa
             st.m = m;
         }
     };
-    int i4 = first + (int)threadIdx.x;
-    for (; i4 + (kAhead - 1) * kBlock < end; i4 += kAhead * kBlock) {
-        f4 v[kAhead];
-#pragma unroll
-        for (int j = 0; j < kAhead; j++) v[j] = __builtin_nontemporal_load(xv + i4 + j * kBlock);
+    auto take = [&](const f4 (&v)[kAhead]) {
         float m = kLowest;
 #pragma unroll
         for (int j = 0; j < kAhead; j++) m = fmaxf(m, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
@@ -781,12 +783,22 @@ __global__ __launch_bounds__(kBlock) void streamed_rows_kernel(Op op, const floa
         for (int j = 0; j < kAhead; j++)
 #pragma unroll
             for (int c = 0; c < 4; c++) add_logit<EXTRA>(st, v[j][c], ks);
-    }
-    for (; i4 < end; i4 += kBlock) {
-        const f4 v = __builtin_nontemporal_load(xv + i4);
-        raise(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+    };
+    int i4 = first + (int)threadIdx.x;
+    for (; i4 + (kAhead - 1) * BLOCK < end; i4 += kAhead * BLOCK) {
+        f4 v[kAhead];
 #pragma unroll
-        for (int c = 0; c < 4; c++) add_logit<EXTRA>(st, v[c], ks);
+        for (int j = 0; j < kAhead; j++) v[j] = __builtin_nontemporal_load(xv + i4 + j * BLOCK);
+        take(v);
+    }
+    if (i4 < end) {                                               // the rest, in flight together as well
+        f4 v[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            v[j] = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (i4 + j * BLOCK < end) v[j] = __builtin_nontemporal_load(xv + i4 + j * BLOCK);
+        }
+        take(v);
     }
     const int64_t single = run == 0 ? sh.single((int)threadIdx.x) : -1;
     if (single >= 0) {
@@ -794,22 +806,21 @@ __global__ __launch_bounds__(kBlock) void streamed_rows_kernel(Op op, const floa
         raise(z);
         add_logit<EXTRA>(st, z, ks);
     }
-    const float m = block_max<kBlock>(st.m, red[0]);
+    const float m = block_max<BLOCK>(st.m, red[0]);
     RowStats o = against<EXTRA>(st, m, ks);
-    if (EXTRA != kNone) block_sum2<kBlock>(o.s, o.x, red[1]);
-    else o.s = block_sum<kBlock>(o.s, red[1]);
-    if (threadIdx.x == 0) runs[row * splits + run] = RowStats{m, o.s, o.x};
+    if (EXTRA != kNone) block_sum2<BLOCK>(o.s, o.x, red[1]);
+    else o.s = block_sum<BLOCK>(o.s, red[1]);
+    if (threadIdx.x == 0) {
+        if (runs) runs[row * splits + run] = RowStats{m, o.s, o.x};
+        else op.template finish<EXTRA>(row, RowStats{m, o.s, o.x}, zt, ListSums{0.0, 0.0, 0.0f});
+    }
 }
 
 template <class Op, int EXTRA>
 __global__ __launch_bounds__(kBlock) void join_runs_kernel(Op op, const float* logits, int64_t rows, int64_t cols, int splits, const RowStats* runs) {
     const int64_t row = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
     const int lane = (int)threadIdx.x & 63;
-    if (row >= rows) return;
-    if (!op.live(row)) {
-        if (lane == 0) op.dead(row);
-        return;
-    }
+    if (row >= rows || !op.live(row)) return;
     const RowStats got = lane < splits ? runs[row * splits + lane] : RowStats{kLowest, 0.0f, 0.0f};
     const float m = wave_top(got.m);
     const RowStats o = against<EXTRA>(got, m, op.k);
@@ -823,17 +834,29 @@ static int streamed_runs(int64_t rows, int64_t cols) {
     const int64_t n = wanted < most ? wanted : most;
     return (int)(n < 1 ? 1 : n > kMaxRuns ? kMaxRuns : n);
 }
+// Few rows, each short enough for one workgroup of 1024 lanes: one launch instead of two.
+static bool in_one_run(int64_t rows, int64_t cols) { return rows <= 256 && cols <= 262144; }
 static size_t streamed_ws_bytes(int64_t rows, int64_t cols) {
-    return rows > 0 && cols > 32768 ? up16((size_t)rows * streamed_runs(rows, cols) * sizeof(RowStats)) : 0;
+    return rows > 0 && cols > 32768 && !in_one_run(rows, cols) ? up16((size_t)rows * streamed_runs(rows, cols) * sizeof(RowStats)) : 0;
+}
+
+template <class Op, int EXTRA>
+static int launch_runs(const Op& op, const float* logits, int64_t rows, int64_t cols, int splits, RowStats* runs, hipStream_t st) {
+    SERAPH_REQUIRE(rows * splits <= 0x7fffffff, "too many rows: %lld", (long long)rows);
+    if (in_one_run(rows, cols))
+        hipLaunchKernelGGL((streamed_rows_kernel<Op, EXTRA, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, op, logits, cols, 1, runs);
+    else
+        hipLaunchKernelGGL((streamed_rows_kernel<Op, EXTRA, kBlock>), dim3((unsigned)(rows * splits)), dim3(kBlock), 0, st, op, logits, cols, splits, runs);
+    SERAPH_LAUNCH_CHECK();
+    return SERAPH_OK;
 }
 
 template <class Op, int EXTRA>
 static int launch_streamed(const Op& op, const float* logits, int64_t rows, int64_t cols, void* ws, hipStream_t st) {
     const int splits = streamed_runs(rows, cols);
-    RowStats* runs = reinterpret_cast<RowStats*>(ws);
-    SERAPH_REQUIRE(rows * splits <= 0x7fffffff, "too many rows: %lld", (long long)rows);
-    hipLaunchKernelGGL((streamed_rows_kernel<Op, EXTRA>), dim3((unsigned)(rows * splits)), dim3(kBlock), 0, st, op, logits, cols, splits, runs);
-    SERAPH_LAUNCH_CHECK();
+    RowStats* runs = in_one_run(rows, cols) ? nullptr : reinterpret_cast<RowStats*>(ws);
+    const int rc = launch_runs<Op, EXTRA>(op, logits, rows, cols, splits, runs, st);
+    if (rc != SERAPH_OK || !runs) return rc;
     hipLaunchKernelGGL((join_runs_kernel<Op, EXTRA>), dim3((unsigned)ceil_div(rows, kBlock / 64)), dim3(kBlock), 0, st, op, logits, rows, cols, splits, runs);
     SERAPH_LAUNCH_CHECK();
     return SERAPH_OK;
@@ -923,75 +946,105 @@ static int launch_rows(const Op& op, const float* logits, float* grad, int64_t r
 }
 
 // ---------------------------------------------------------------- preference pairs
+// Every row's factor follows from both sequences of its pair, so the logits are read twice: once for the rows' statistics,
+// once for the gradient, which then is a streaming pass without any reduction.
 struct PreferenceArgs {
+    const float* logits;
+    const uint32_t* targets;
     const float* ref_logp;
-    float *loss_pairs, *scores, *logp_rows;
     const uint32_t* seq_starts;
-    int pairs;
-    int64_t rows;
-    int kind, average;
+    const RowStats* runs;          // `splits` results for each supervised row; where it is one, x is the target's logit
+    float *loss_pairs, *scores, *logp_rows;
+    int64_t rows, cols;
+    int pairs, splits, kind, average;
     float beta, smoothing, margin;
 };
 
 // What the gradient pass needs of a row: its maximum, the factor of exp(z - m), and what the target takes off.
+constexpr uint32_t kDead = 0xffffffffu;
 struct RowFactor { float m, a, c; uint32_t target; };
-struct RowTotals { float m, s; };
 
-// The statistics of the supervised rows; logp in 64 bits, because a score is a difference of long sums.
 struct PairRowsOp {
     static constexpr bool kGrad = false, kList = false;
     Supervision rows;
-    RowTotals* totals;
-    double* logp;
-    RowFactor* factors;
+    RowStats* runs;
+    RowFactor* factors;            // NULL: not wanted
     float* logp_rows;
     ExpScale k;
     __device__ __forceinline__ bool live(int64_t r) const { return rows.live(r); }
     __device__ __forceinline__ int64_t target(int64_t r) const { return rows.targets[r]; }
     __device__ __forceinline__ void dead(int64_t r) const {
-        totals[r] = RowTotals{0.0f, 0.0f};
-        factors[r] = RowFactor{0.0f, 0.0f, 0.0f, 0xffffffffu};    // target: the row is not supervised
-        logp[r] = 0.0;
+        if (factors) factors[r] = RowFactor{0.0f, 0.0f, 0.0f, kDead};
         if (logp_rows) logp_rows[r] = 0.0f;
     }
     template <int EXTRA>
-    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&, bool writes = true) const {
-        const double v = ((double)zt - (double)st.m) - log((double)st.s);
-        totals[r] = RowTotals{st.m, st.s};
-        factors[r] = RowFactor{st.m, 0.0f, 0.0f, rows.targets[r]};
-        logp[r] = v;
-        if (logp_rows) logp_rows[r] = (float)v;
+    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&) const {
+        runs[r] = RowStats{st.m, st.s, zt};
         return RowGrad{0.0f, 0.0f, 0.0f, -1};
     }
 };
 
-// One workgroup per pair: the two scores, the loss, and the factor of every row of the pair.
-__global__ __launch_bounds__(kBlock) void pair_kernel(PreferenceArgs p, const RowTotals* totals, const double* logp, RowFactor* factors) {
-    __shared__ double red[2][kBlock / 64];
-    __shared__ double red_n[2][kBlock / 64];
-    const int pair = blockIdx.x;
-    double score[2], count[2];
-    int64_t first[2], last[2];
-    for (int side = 0; side < 2; side++) {
-        const uint32_t* b = p.seq_starts + 2 * (int64_t)pair + side;
-        first[side] = b[0];
-        last[side] = (int64_t)b[1] < p.rows ? (int64_t)b[1] : p.rows;
-        double sum = 0.0, n = 0.0;
-        for (int64_t r = first[side] + threadIdx.x; r < last[side]; r += kBlock)
-            if (factors[r].target != 0xffffffffu) {
-                sum += p.ref_logp ? logp[r] - (double)p.ref_logp[r] : logp[r];
-                n += 1.0;
-            }
-        score[side] = block_sum<kBlock>(sum, red[side]);
-        count[side] = block_sum<kBlock>(n, red_n[side]);
-        if (p.average && count[side] > 0.0) score[side] /= count[side];
+__device__ __forceinline__ RowStats joined(const PreferenceArgs& p, int64_t r) {
+    RowStats st = p.runs[r * p.splits];
+    for (int i = 1; i < p.splits; i++) {
+        const RowStats o = p.runs[r * p.splits + i];
+        const float m = fmaxf(st.m, o.m);
+        st = RowStats{m, against<kNone>(st, m, kUnitScale).s + against<kNone>(o, m, kUnitScale).s, 0.0f};
     }
-    const double beta = (double)p.beta, gap = score[0] - score[1], h = beta * gap - (double)p.margin;
-    double loss, slope;                                           // slope: d loss / d gap
+    return st;
+}
+__device__ __forceinline__ RowFactor factor_of(const PreferenceArgs& p, int64_t r, uint32_t target, double f) {
+    const RowStats st = joined(p, r);
+    return RowFactor{st.m, (float)(-f / (double)st.s), (float)-f, target};
+}
+
+// The two sequences of a pair, their scores and its loss; slope0 and slope1 are d(mean loss) / d(log-probability of a token) of
+// either side.  Called by a whole workgroup, half of which sums each side; sums in 64 bits and in one order whoever forms them.
+struct Pair { int64_t first, last, end; double slope0, slope1; };           // first, last, end: of this half's sequence
+template <int BLOCK>
+__device__ __forceinline__ Pair read_pair(const PreferenceArgs& p, int pair, double (*red)[BLOCK / 64], bool writes) {
+    Pair q;
+    const int side = (int)threadIdx.x / (BLOCK / 2);
+    const uint32_t* b = p.seq_starts + 2 * (int64_t)pair + side;
+    q.first = b[0];
+    q.end = b[1];
+    q.last = q.end < p.rows ? q.end : p.rows;
+    double sum = 0.0, n = 0.0;
+    for (int64_t r = q.first + (int)threadIdx.x % (BLOCK / 2); r < q.last; r += BLOCK / 2) {
+        const uint32_t t = p.targets[r];
+        const RowStats st = joined(p, r);                         // (not yet known to hold anything: the loads of a row do not wait for each other)
+        const float ref = p.ref_logp ? p.ref_logp[r] : 0.0f;
+        if ((int64_t)t >= p.cols || r + 1 >= q.end) continue;
+        const float zt = p.splits == 1 ? st.x : p.logits[r * p.cols + t];
+        const double logp = ((double)zt - (double)st.m) - log((double)st.s);
+        if (writes && p.logp_rows) p.logp_rows[r] = (float)logp;
+        sum += logp - (double)ref;
+        n += 1.0;
+    }
+    sum = wave_total(sum);
+    n = wave_total(n);
+    if ((threadIdx.x & 63) == 0) {
+        red[0][threadIdx.x >> 6] = sum;
+        red[1][threadIdx.x >> 6] = n;
+    }
+    __syncthreads();
+    double score0 = 0.0, score1 = 0.0, count0 = 0.0, count1 = 0.0, loss;
+#pragma unroll
+    for (int w = 0; w < BLOCK / 128; w++) {
+        score0 += red[0][w];
+        count0 += red[1][w];
+        score1 += red[0][w + BLOCK / 128];
+        count1 += red[1][w + BLOCK / 128];
+    }
+    if (!p.average || count0 == 0.0) count0 = 1.0;
+    if (!p.average || count1 == 0.0) count1 = 1.0;
+    score0 /= count0;
+    score1 /= count1;
+    const double beta = (double)p.beta, gap = score0 - score1, h = beta * gap - (double)p.margin;
+    double slope;                                                 // d loss / d gap
     if (p.kind == SERAPH_PREFERENCE_SIGMOID) {
         const double eps = (double)p.smoothing, soft = log1p(exp(-fabs(h)));
-        loss = (1.0 - eps) * (soft + fmax(-h, 0.0)) + eps * (soft + fmax(h, 0.0));
-        if (h != h) loss = h;
+        loss = h != h ? h : (1.0 - eps) * (soft + fmax(-h, 0.0)) + eps * (soft + fmax(h, 0.0));
         slope = beta * (eps - 1.0 / (1.0 + exp(h)));
     } else if (p.kind == SERAPH_PREFERENCE_HINGE) {
         loss = h >= 1.0 ? 0.0 : 1.0 - h;
@@ -1001,66 +1054,80 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PreferenceArgs p, const Ro
         loss = d * d;
         slope = 2.0 * d;
     }
-    if (threadIdx.x == 0) {
+    q.slope0 = slope / (double)p.pairs / count0;
+    q.slope1 = -slope / (double)p.pairs / count1;
+    if (writes && threadIdx.x == 0) {
         p.loss_pairs[pair] = (float)loss;
         if (p.scores) {
-            p.scores[2 * (int64_t)pair] = (float)score[0];
-            p.scores[2 * (int64_t)pair + 1] = (float)score[1];
+            p.scores[2 * (int64_t)pair] = (float)score0;
+            p.scores[2 * (int64_t)pair + 1] = (float)score1;
         }
     }
-    for (int side = 0; side < 2; side++) {
-        const double f = (side ? -slope : slope) / (double)p.pairs / (p.average && count[side] > 0.0 ? count[side] : 1.0);
-        for (int64_t r = first[side] + threadIdx.x; r < last[side]; r += kBlock)
-            if (factors[r].target != 0xffffffffu) {
-                factors[r].a = (float)(-f / (double)totals[r].s);
-                factors[r].c = (float)-f;
-            }
+    return q;
+}
+
+constexpr int kPairBlock = 512;
+
+// One workgroup per pair writes the factors of its rows (those that are not supervised have been marked by the pass before).
+__global__ __launch_bounds__(1024) void pair_kernel(PreferenceArgs p, RowFactor* factors) {
+    __shared__ double red[2][1024 / 64];
+    const Pair q = read_pair<1024>(p, (int)blockIdx.x, red, true);
+    const double f = threadIdx.x < 512 ? q.slope0 : q.slope1;
+    for (int64_t r = q.first + (int)threadIdx.x % 512; r < q.last; r += 512) {
+        const uint32_t t = p.targets[r];
+        if ((int64_t)t < p.cols && r + 1 < q.end) factors[r] = factor_of(p, r, t, f);
     }
 }
 
-// One workgroup per run of kPairVpt vectors per lane of a row; the rows are walked back from the last one, whose logits the
-// pass before this one has left in the last-level cache.
-constexpr int kPairVpt = 8;
-__global__ __launch_bounds__(kBlock) void pair_grad_kernel(const float* logits, float* grad, const RowFactor* factors, int64_t rows, int64_t cols, int runs) {
-    const int64_t row = rows - 1 - (int64_t)(blockIdx.x / (unsigned)runs);
-    const int run = (int)(blockIdx.x % (unsigned)runs);
-    const RowFactor f = factors[row];
-    const float* x = logits + row * cols;
-    float* out = grad + row * cols;
-    const RowShape sh(x, cols);
-    const f4* xv = reinterpret_cast<const f4*>(x + sh.head);
-    f4a4* ov = reinterpret_cast<f4a4*>(out + sh.head);
-    const int first = run * kPairVpt * kBlock + (int)threadIdx.x;
+// One vector per lane: of all shapes tried (1 to 16 vectors per lane, 128 to 1024 lanes, either order of the rows) the smallest
+// pieces of work keep reads and writes best mixed: 4096 x 151936 in 0.80 ms (6.2 TB/s), with eight vectors 0.92 ms.
+__device__ __forceinline__ void pair_grad(const PreferenceArgs& p, float* grad, int64_t row, int run, const RowFactor& f) {
+    const float* x = p.logits + row * p.cols;
+    float* out = grad + row * p.cols;
+    const RowShape sh(x, p.cols);
+    const int i4 = run * kPairBlock + (int)threadIdx.x;
     const int64_t single = run == 0 ? sh.single((int)threadIdx.x) : -1;
-    if (f.target == 0xffffffffu) {
-#pragma unroll
-        for (int j = 0; j < kPairVpt; j++)
-            if (first + j * kBlock < sh.n4) ov[first + j * kBlock] = f4{0, 0, 0, 0};
+    f4a4* to = reinterpret_cast<f4a4*>(out + sh.head) + i4;
+    if (f.target == kDead) {
+        if (i4 < sh.n4) __builtin_nontemporal_store(f4a4{0, 0, 0, 0}, to);
         if (single >= 0) out[single] = 0.0f;
         return;
     }
-    const int tv = (int)f.target - sh.head, t4 = (int)f.target >= sh.head ? tv >> 2 : -1;
-    const f4 off_target = {(tv & 3) == 0 ? f.c : 0.0f, (tv & 3) == 1 ? f.c : 0.0f, (tv & 3) == 2 ? f.c : 0.0f, (tv & 3) == 3 ? f.c : 0.0f};
-    f4 v[kPairVpt];
+    if (i4 < sh.n4) {
+        const f4 v = __builtin_nontemporal_load(reinterpret_cast<const f4*>(x + sh.head) + i4);
+        const int c = (int)f.target - (sh.head + i4 * 4);
+        f4a4 r;
 #pragma unroll
-    for (int j = 0; j < kPairVpt; j++)
-        if (first + j * kBlock < sh.n4) v[j] = __builtin_nontemporal_load(xv + first + j * kBlock);
-    const float one = single >= 0 ? x[single] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < kPairVpt; j++) {
-        const int i4 = first + j * kBlock;
-        if (i4 < sh.n4) {
-            f4 r;
-#pragma unroll
-            for (int c = 0; c < 4; c++) r[c] = f.a * exp_of(v[j][c], f.m, kUnitScale);
-            if (i4 == t4) r -= off_target;
-            __builtin_nontemporal_store((f4a4)r, ov + i4);
-        }
+        for (int j = 0; j < 4; j++) r[j] = f.a * exp_of(v[j], f.m, kUnitScale) - (j == c ? f.c : 0.0f);
+        __builtin_nontemporal_store(r, to);
     }
-    if (single >= 0) {
-        const float r = f.a * exp_of(one, f.m, kUnitScale);
-        out[single] = single == (int64_t)f.target ? r - f.c : r;
+    if (single >= 0) out[single] = f.a * exp_of(x[single], f.m, kUnitScale) - (single == (int64_t)f.target ? f.c : 0.0f);
+}
+
+__global__ __launch_bounds__(kPairBlock) void pair_grad_kernel(PreferenceArgs p, float* grad, const RowFactor* factors, int splits_of_row) {
+    const int64_t row = (int64_t)(blockIdx.x / (unsigned)splits_of_row);
+    pair_grad(p, grad, row, (int)(blockIdx.x % (unsigned)splits_of_row), factors[row]);
+}
+
+// A batch whose gradient is a single round of workgroups: each reads its row's pair by itself, which takes less than the launch
+// it replaces.  `pairs` further workgroups write the pairs' own results.  (In place too: the targets' logits have been
+// kept by the pass before, and every other logit is read by the workgroup that overwrites it.)
+__global__ __launch_bounds__(kPairBlock) void small_pairs_kernel(PreferenceArgs p, float* grad, int splits_of_row) {
+    __shared__ double red[2][kPairBlock / 64];
+    const int64_t row = (int64_t)(blockIdx.x / (unsigned)splits_of_row);
+    const int run = (int)(blockIdx.x % (unsigned)splits_of_row);
+    if (row >= p.rows) {
+        read_pair<kPairBlock>(p, (int)(blockIdx.x - (unsigned)(p.rows * splits_of_row)), red, true);
+        return;
     }
+    RowFactor f{0.0f, 0.0f, 0.0f, kDead};
+    const int sq = find_seq(p.seq_starts, 2 * p.pairs, row);
+    const uint32_t t = p.targets[row];
+    if (sq < 2 * p.pairs && row + 1 < (int64_t)p.seq_starts[sq + 1] && (int64_t)t < p.cols) {
+        const Pair q = read_pair<kPairBlock>(p, sq / 2, red, false);
+        f = factor_of(p, row, t, sq & 1 ? q.slope1 : q.slope0);
+    }
+    pair_grad(p, grad, row, run, f);
 }
 
 }  // namespace seraph
@@ -1122,10 +1189,10 @@ int seraph_policy_grad(const float* logits, const uint32_t* actions, const float
     return launch_rows<PolicyOp, kNone>(op, logits, grad, rows, cols, 0, ws, as_stream(s));
 }
 
+static int pair_runs(int64_t rows, int64_t cols) { return cols <= 32768 || in_one_run(rows, cols) ? 1 : streamed_runs(rows, cols); }
 size_t seraph_preference_grad_ws_bytes(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    return up16((size_t)rows * sizeof(RowFactor)) + up16((size_t)rows * sizeof(double)) + up16((size_t)rows * sizeof(RowTotals)) +
-           streamed_ws_bytes(rows, cols);
+    return up16((size_t)rows * sizeof(RowFactor)) + up16((size_t)rows * pair_runs(rows, cols) * sizeof(RowStats));
 }
 
 int seraph_preference_grad(const float* logits, const uint32_t* targets, const float* ref_logp, float* grad,
@@ -1142,20 +1209,26 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
     SERAPH_REQUIRE(isfinite(options->margin), "preference_grad: margin must be finite");
     REQUIRE_WS("preference_grad", seraph_preference_grad_ws_bytes(rows, cols));
     hipStream_t st = as_stream(s);
-    char* p = reinterpret_cast<char*>(ws);
-    RowFactor* factors = reinterpret_cast<RowFactor*>(p);
-    double* logp = reinterpret_cast<double*>(p += up16((size_t)rows * sizeof(RowFactor)));
-    RowTotals* totals = reinterpret_cast<RowTotals*>(p += up16((size_t)rows * sizeof(double)));
-    PairRowsOp op{{targets, nullptr, seq_starts, 2 * pairs, cols}, totals, logp, factors, logp_rows, kUnitScale};
-    const int rc = launch_rows<PairRowsOp, kNone>(op, logits, nullptr, rows, cols, 0, p + up16((size_t)rows * sizeof(RowTotals)), st);
+    const int splits = pair_runs(rows, cols);
+    RowFactor* factors = reinterpret_cast<RowFactor*>(ws);
+    RowStats* runs = reinterpret_cast<RowStats*>(reinterpret_cast<char*>(ws) + up16((size_t)rows * sizeof(RowFactor)));
+    const int64_t row_splits = ceil_div(ceil_div(cols, 4), kPairBlock);
+    SERAPH_REQUIRE(rows * row_splits <= 0x7fffffff, "preference_grad: too many logits: %lld x %lld", (long long)rows, (long long)cols);
+    const bool small = splits == 1 && rows * row_splits + pairs <= 4 * (int64_t)num_compute_units();      // four workgroups of 512 lanes on a CU
+    PairRowsOp op{{targets, nullptr, seq_starts, 2 * pairs, cols}, runs, small ? nullptr : factors, logp_rows, kUnitScale};
+    const int rc = cols <= 32768 ? launch_rows<PairRowsOp, kNone>(op, logits, nullptr, rows, cols, 0, nullptr, st)
+                                 : launch_runs<PairRowsOp, kNone>(op, logits, rows, cols, splits, splits == 1 ? nullptr : runs, st);
     if (rc != SERAPH_OK) return rc;
-    PreferenceArgs a{ref_logp, loss_pairs, scores, logp_rows, seq_starts, pairs, rows, options->kind, options->average,
-                     options->beta, options->label_smoothing, options->margin};
-    hipLaunchKernelGGL(pair_kernel, dim3((unsigned)pairs), dim3(kBlock), 0, st, a, totals, logp, factors);
+    const PreferenceArgs a{logits, targets, ref_logp, seq_starts, runs, loss_pairs, scores, logp_rows, rows, cols, pairs, splits,
+                           options->kind, options->average, options->beta, options->label_smoothing, options->margin};
+    if (small) {
+        hipLaunchKernelGGL(small_pairs_kernel, dim3((unsigned)(rows * row_splits + pairs)), dim3(kPairBlock), 0, st, a, grad, (int)row_splits);
+        SERAPH_LAUNCH_CHECK();
+        return SERAPH_OK;
+    }
+    hipLaunchKernelGGL(pair_kernel, dim3((unsigned)pairs), dim3(1024), 0, st, a, factors);
     SERAPH_LAUNCH_CHECK();
-    const int64_t runs = ceil_div(ceil_div(cols, 4), kPairVpt * kBlock);
-    SERAPH_REQUIRE(rows * runs <= 0x7fffffff, "preference_grad: too many logits: %lld x %lld", (long long)rows, (long long)cols);
-    hipLaunchKernelGGL(pair_grad_kernel, dim3((unsigned)(rows * runs)), dim3(kBlock), 0, st, logits, grad, factors, rows, cols, (int)runs);
+    hipLaunchKernelGGL(pair_grad_kernel, dim3((unsigned)(rows * row_splits)), dim3(kPairBlock), 0, st, a, grad, factors, (int)row_splits);
     SERAPH_LAUNCH_CHECK();
     return SERAPH_OK;
 }
