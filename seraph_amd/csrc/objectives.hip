@@ -834,8 +834,10 @@ static int streamed_runs(int64_t rows, int64_t cols) {
     const int64_t n = wanted < most ? wanted : most;
     return (int)(n < 1 ? 1 : n > kMaxRuns ? kMaxRuns : n);
 }
-// Few rows, each short enough for one workgroup of 1024 lanes: one launch instead of two.
-static bool in_one_run(int64_t rows, int64_t cols) { return rows <= 256 && cols <= 262144; }
+// Few rows, each short enough for one workgroup of 1024 lanes: one launch instead of two.  One CU takes 11.4 us for the
+// exponentials of 151936 columns, which is what the second launch costs (8 rows: 11.4 us against 12.2 us in a sequence of calls);
+// longer rows are better cut.
+static bool in_one_run(int64_t rows, int64_t cols) { return rows <= 256 && cols <= 163840; }
 static size_t streamed_ws_bytes(int64_t rows, int64_t cols) {
     return rows > 0 && cols > 32768 && !in_one_run(rows, cols) ? up16((size_t)rows * streamed_runs(rows, cols) * sizeof(RowStats)) : 0;
 }

@@ -93,10 +93,10 @@ def _expect(op, name, t, dtypes, shape, device):
     """The address of an argument after its type, shape, layout and device have been checked; None for None."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        got = f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise SeraphError(f"{op}: {name} has to be contiguous {'/'.join(str(d) for d in dtypes)} {shape} on {device}; got {got}")
-    return t.data_ptr()
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.shape == shape and t.is_contiguous() and t.device == device:
+        return t.data_ptr()
+    got = f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}" if isinstance(t, torch.Tensor) else type(t).__name__
+    raise SeraphError(f"{op}: {name} has to be contiguous {'/'.join(str(d) for d in dtypes)} {shape} on {device}; got {got}")
 
 
 _F32 = (torch.float32,)
@@ -129,23 +129,13 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class _on:
-    """Makes `device` the current one for a call, where it is not, and gives the handle of its current stream (without
-    the stream object around it, whose construction takes as long as a launch)."""
-
-    def __init__(self, device):
-        self.device, self.before = device.index, None
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        if now != self.device:
-            self.before = now
-            torch.cuda.set_device(self.device)
-        return torch._C._cuda_getCurrentRawStream(self.device)
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+def _call(op, device, entry, *args):
+    """entry(*args, stream) on the current stream of `device`, which is made the current device where it is not.  (The
+    stream's handle alone: the object around it takes as long to make as a launch.)"""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return check(entry(*args, torch._C._cuda_getCurrentRawStream(device.index)), op)
+    check(entry(*args, torch._C._cuda_getCurrentRawStream(device.index)), op)
 
 
 def token_logprobs(logits, targets, seq_starts=None, want_lse=False, want_entropy=False):
@@ -160,9 +150,8 @@ def token_logprobs(logits, targets, seq_starts=None, want_lse=False, want_entrop
     k = kernels()
     nbytes = k.seraph_token_logprobs_ws_bytes(rows, cols)
     ws = _scratch(nbytes, device)
-    with _on(device) as stream:
-        check(k.seraph_token_logprobs(logits.data_ptr(), t, logp.data_ptr(), _ptr(lse), _ptr(entropy), st, batch, rows, cols,
-                                      _ptr(ws), nbytes, stream), op)
+    _call(op, device, k.seraph_token_logprobs, logits.data_ptr(), t, logp.data_ptr(), _ptr(lse), _ptr(entropy), st, batch, rows, cols,
+          _ptr(ws), nbytes)
     return logp, lse, entropy
 
 
@@ -187,9 +176,8 @@ def policy_grad(logits, actions, advantages, old_logp, valid_rows, ref_logp=None
     nbytes = k.seraph_policy_grad_ws_bytes(rows, cols)
     ws = _scratch(nbytes, device)
     options = PolicyOptions(clip[0], clip[1], kl_coef, entropy_coef)
-    with _on(device) as stream:
-        check(k.seraph_policy_grad(logits.data_ptr(), a, adv, old, ref, w, g, loss.data_ptr(), logp.data_ptr(), _ptr(kl), _ptr(entropy),
-                                   options, st, batch, rows, cols, valid_rows, _ptr(ws), nbytes, stream), op)
+    _call(op, device, k.seraph_policy_grad, logits.data_ptr(), a, adv, old, ref, w, g, loss.data_ptr(), logp.data_ptr(), _ptr(kl), _ptr(entropy),
+          options, st, batch, rows, cols, valid_rows, _ptr(ws), nbytes)
     return grad, loss, logp, kl, entropy
 
 
@@ -215,9 +203,8 @@ def preference_grad(logits, targets, seq_starts, ref_logp=None, kind="sigmoid", 
     nbytes = k.seraph_preference_grad_ws_bytes(rows, cols)
     ws = _scratch(nbytes, device)
     options = PreferenceOptions(PREFERENCE_KINDS[kind], beta, label_smoothing, margin, 1 if average else 0)
-    with _on(device) as stream:
-        check(k.seraph_preference_grad(logits.data_ptr(), t, ref, g, loss.data_ptr(), scores.data_ptr(), None, options, st, batch // 2,
-                                       rows, cols, _ptr(ws), nbytes, stream), op)
+    _call(op, device, k.seraph_preference_grad, logits.data_ptr(), t, ref, g, loss.data_ptr(), scores.data_ptr(), None, options, st, batch // 2,
+          rows, cols, _ptr(ws), nbytes)
     return grad, loss, scores
 
 
@@ -242,9 +229,8 @@ def distill_grad(logits, teacher_ids, teacher_logits, valid_rows, temperature=1.
     nbytes = k.seraph_distill_grad_ws_bytes(rows, cols, top_k)
     ws = _scratch(nbytes, device)
     options = DistillOptions(temperature, soft_coef, hard_coef, TEACHER_TYPES[teacher_logits.dtype])
-    with _on(device) as stream:
-        check(k.seraph_distill_grad(logits.data_ptr(), ids, tl, tlse, t, w, g, loss.data_ptr(), options, st, batch, rows, cols, top_k,
-                                    valid_rows, _ptr(ws), nbytes, stream), op)
+    _call(op, device, k.seraph_distill_grad, logits.data_ptr(), ids, tl, tlse, t, w, g, loss.data_ptr(), options, st, batch, rows, cols, top_k,
+          valid_rows, _ptr(ws), nbytes)
     return grad, loss
 
 
