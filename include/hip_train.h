@@ -28,6 +28,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include "seraph_hip.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -112,6 +114,30 @@ float hip_eval_forward_batch(hip_trainer_t* t, const int* tokens_packed, int tot
                              const int* seq_starts, int batch_size);
 float hip_evaluate(hip_trainer_t* t, const int* val_tokens, int num_val_tokens, const int* offsets, int num_samples,
                    int max_seq_len, int max_eval_samples, float* out_perplexity);
+
+/* Steps with another objective, full-weight or LoRA as the trainer is: the same forward, backward, optimizer and bookkeeping,
+ * with seraph_policy_grad, seraph_preference_grad or seraph_distill_grad (seraph_hip.h has their formulas and options) in
+ * the place of the cross entropy.  The reference has no counterpart.  Arrays per token are HOST arrays of total_tokens
+ * entries; entry r belongs to the prediction made at token r, whose target is token r + 1 of its sequence (entries of
+ * a sequence's last token are ignored).  A prediction whose weight, or whose `supervised` byte, is 0 does not count:
+ * mark prompts so.  Policy and distillation losses are the sum over the predictions that count, divided by their number.
+ * Return 0 and the loss, which may be negative, in *loss (NAN where the NaN check stopped the step); -1 on error.  A batch
+ * without a prediction that counts changes nothing and has the loss 0 (a preference step still steps).
+ *
+ * hip_token_logprobs is the pass that policy and reference log-probabilities come from: forward only, one value for each
+ * prediction (0 for the last token of a sequence), entropy optional.  use_adapters = 0 leaves the adapters of a LoRA
+ * trainer out: its frozen base model is the reference of its own fine-tuning. */
+int hip_token_logprobs(hip_trainer_t* t, const int* tokens_packed, int total_tokens, const int* seq_starts, int batch_size,
+                       int use_adapters, float* logp, float* entropy);
+int hip_train_step_policy(hip_trainer_t* t, const int* tokens_packed, int total_tokens, const int* seq_starts, int batch_size,
+                          const float* advantages, const float* old_logp, const float* ref_logp, const float* weights,
+                          const seraph_policy_options_t* options, int run_optimizer, float* loss);
+int hip_train_step_preference(hip_trainer_t* t, const int* tokens_packed, int total_tokens, const int* seq_starts, int pairs,
+                              const uint8_t* supervised, const float* ref_logp, const seraph_preference_options_t* options,
+                              int run_optimizer, float* loss, float* scores);
+int hip_train_step_distill(hip_trainer_t* t, const int* tokens_packed, int total_tokens, const int* seq_starts, int batch_size,
+                           const uint32_t* teacher_ids, const void* teacher_logits, const float* teacher_lse, int top_k,
+                           const float* weights, const seraph_distill_options_t* options, int run_optimizer, float* loss);
 
 /* Resume support: the learning rate and the two counters of src/train.c:5439-5463
  * (state->optimizer_step, state->accumulation_counter); a negative counter is left unchanged. */

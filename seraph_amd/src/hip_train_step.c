@@ -70,6 +70,8 @@ struct hip_trainer {
     void* attn_ws;               /* attention-backward scratch incl. the dS band; grown to the longest sequence seen */
     size_t attn_ws_bytes;
     int64_t max_seq_len;         /* of the current batch */
+    void* obj_dev;               /* inputs, results and scratch of a step with another objective; grown to the largest seen */
+    size_t obj_bytes;
     size_t device_bytes;
     /* bookkeeping of src/train.c:5439-5463 */
     int accumulation_counter, optimizer_step;
@@ -463,6 +465,7 @@ void hip_trainer_free(hip_trainer_t* t) {
     seraph_hip_free(t->norm_parts);
     free(t->norm_jobs);
     seraph_hip_free(t->attn_ws);
+    seraph_hip_free(t->obj_dev);
     seraph_hip_free(t->d_nan_flags);
     free(t->h_nan_flags);
     seraph_hip_host_free(t->h_stage);
@@ -634,7 +637,74 @@ static int lora_backward_group(hip_trainer_t* t, const lora_bwd_item_t* it, int 
     return 0;
 }
 
-static int upload_batch(hip_trainer_t* t, const int* tokens, int T, const int* seq_starts, int batch) {
+/* What a step learns where that is not the next token (NULL: the cross entropy).  Arrays per token follow the loss rows:
+ * entry r belongs to the prediction made at token r, whose target is token r + 1 of the same sequence. */
+enum { OBJ_LOGPROBS, OBJ_POLICY, OBJ_PREFERENCE, OBJ_DISTILL };
+typedef struct {
+    int kind, frozen;                /* frozen: forward without the adapters */
+    const uint8_t* supervised;       /* host inputs, NULL where the objective has none */
+    const float *weights, *advantages, *old_logp, *ref_logp, *teacher_lse;
+    const uint32_t* teacher_ids;
+    const void* teacher_logits;
+    int64_t top_k;
+    const seraph_policy_options_t* policy;
+    const seraph_preference_options_t* preference;
+    const seraph_distill_options_t* distill;
+    float *host_logp, *host_entropy, *host_scores;
+    float loss;
+    /* device copies, results and scratch */
+    float *d_weights, *d_advantages, *d_old, *d_ref, *d_teacher_lse, *d_logp, *d_entropy, *d_scores;
+    uint32_t* d_ids;
+    void *d_teacher, *ws;
+    size_t ws_bytes;
+} objective_t;
+
+static int row_supervised(const objective_t* o, uint32_t r) {
+    return (!o->supervised || o->supervised[r]) && (!o->weights || o->weights[r] != 0.0f);
+}
+
+/* device room for everything an objective needs beside the logits, and its inputs in it */
+static int upload_objective(hip_trainer_t* t, objective_t* o, int T, int batch) {
+    const size_t row = up256((size_t)T * 4), V = (size_t)t->cfg.vocab;
+    const size_t list = up256((size_t)T * (size_t)o->top_k * 4);
+    o->ws_bytes = o->kind == OBJ_LOGPROBS ? seraph_token_logprobs_ws_bytes(T, (int64_t)V) :
+                  o->kind == OBJ_POLICY ? seraph_policy_grad_ws_bytes(T, (int64_t)V) :
+                  o->kind == OBJ_PREFERENCE ? seraph_preference_grad_ws_bytes(T, (int64_t)V) :
+                  seraph_distill_grad_ws_bytes(T, (int64_t)V, o->top_k);
+    const size_t need = 7 * row + up256((size_t)batch * 4) + 2 * list + up256(o->ws_bytes);
+    if (need > t->obj_bytes) {
+        CK(seraph_hip_stream_sync(t->stream));
+        if (t->obj_dev) { seraph_hip_free(t->obj_dev); t->device_bytes -= t->obj_bytes; t->obj_dev = NULL; t->obj_bytes = 0; }
+        if (dev_alloc(t, &t->obj_dev, need)) return -1;
+        t->obj_bytes = need;
+    }
+    char* p = (char*)t->obj_dev;
+#define ROOM(dst, bytes) do { (dst) = (void*)p; p += up256(bytes); } while (0)
+#define GIVE(dst, src, bytes)                                                                    \
+    do {                                                                                         \
+        void* at_ = NULL;                                                                        \
+        ROOM(at_, (bytes));                                                                      \
+        (dst) = (src) ? at_ : NULL;                                                              \
+        if (src) CK(seraph_hip_h2d(at_, (src), (bytes), t->stream));                             \
+    } while (0)
+    const size_t rb = (size_t)T * 4;
+    GIVE(o->d_weights, o->weights, rb);
+    GIVE(o->d_advantages, o->advantages, rb);
+    GIVE(o->d_old, o->old_logp, rb);
+    GIVE(o->d_ref, o->ref_logp, rb);
+    GIVE(o->d_teacher_lse, o->teacher_lse, rb);
+    ROOM(o->d_logp, rb);
+    ROOM(o->d_entropy, rb);
+    ROOM(o->d_scores, (size_t)batch * 4);
+    GIVE(o->d_ids, o->teacher_ids, (size_t)T * (size_t)o->top_k * 4);
+    GIVE(o->d_teacher, o->teacher_logits, (size_t)T * (size_t)o->top_k * (o->distill && o->distill->teacher_type != SERAPH_TYPE_F32 ? 2 : 4));
+    o->ws = p;
+#undef GIVE
+#undef ROOM
+    return 0;
+}
+
+static int upload_batch(hip_trainer_t* t, const int* tokens, int T, const int* seq_starts, int batch, const objective_t* obj) {
     uint32_t* tok = t->h_stage;
     uint32_t* tgt = tok + T;
     uint32_t* st = tgt + T;
@@ -649,6 +719,7 @@ static int upload_batch(hip_trainer_t* t, const int* tokens, int T, const int* s
         for (uint32_t i = st[b]; i < st[b + 1]; i++) {                     /* src/train_cuda.c:2029-2043 */
             tok[i] = tokens[i] < 0 ? 0u : (uint32_t)tokens[i];
             tgt[i] = (i + 1 < st[b + 1]) ? (tokens[i + 1] < 0 ? 0u : (uint32_t)tokens[i + 1]) : 0u;
+            if (obj && !row_supervised(obj, i)) tgt[i] = 0xffffffffu;
         }
     }
     /* attention-backward scratch: the dS band for this batch's longest sequence when it stays under
@@ -760,8 +831,9 @@ static void nan_dump(hip_trainer_t* t, int total_tokens) {
 
 enum { STEP_TRAIN = 0, STEP_EVAL = 1 };
 
+/* The mean loss, or with an objective 0 and its own loss in obj->loss; -1 on error, NAN where the NaN check stopped the step. */
 static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, const int* seq_starts, int batch,
-                      int run_optimizer, int mode) {
+                      int run_optimizer, int mode, objective_t* obj) {
     if (!t || !tokens || total_tokens < 2 || batch < 1) return -1.0f;
     if (total_tokens > t->max_tokens || batch > t->max_batch) {
         fprintf(stderr, "ERROR: batch of %d tokens / %d sequences exceeds the trainer's capacity (%d / %d)\n",
@@ -776,13 +848,23 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
     const int64_t qd = (int64_t)H * D, kv = (int64_t)KVH * D;
     const float scale = 1.0f / sqrtf((float)D);
     const float eps = c->rms_eps, theta = c->rope_theta > 0 ? c->rope_theta : 10000.0f;
-    const int num_valid = total_tokens - batch;                         /* src/train_cuda.c:1989-1991 */
+    int num_valid = total_tokens - batch;                               /* src/train_cuda.c:1989-1991 */
     if (num_valid <= 0) return 0.0f;
+    if (obj && obj->kind != OBJ_LOGPROBS) {                             /* the predictions that count: not the prompts', not a sequence's last */
+        num_valid = 0;
+        for (int b = 0; b < batch; b++) {
+            const int from = seq_starts ? seq_starts[b] : 0, to = seq_starts ? seq_starts[b + 1] : total_tokens;
+            for (int r = from < 0 ? 0 : from; r + 1 < to && r < total_tokens; r++) num_valid += row_supervised(obj, (uint32_t)r);
+        }
+        if (num_valid == 0 && obj->kind != OBJ_PREFERENCE) return 0.0f;
+    }
     seraph_stream_t s = t->stream;
     const float* P = t->P;
 
     seraph_hip_event_on_next_op(NULL);      /* an event this thread armed before the step belongs to none of its ops */
-    if (upload_batch(t, tokens, total_tokens, seq_starts, batch)) return -1.0f;
+    if (upload_batch(t, tokens, total_tokens, seq_starts, batch, obj)) return -1.0f;
+    if (obj && upload_objective(t, obj, total_tokens, batch)) return -1.0f;
+    const int adapters = lora && !(obj && obj->frozen);
     const uint32_t* starts = t->d_starts;
 
     /* flag indices, src/train.c:4499-4537 */
@@ -805,7 +887,7 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
     NANCHK(t->act[0].layer_in, T * h, 7u);
     for (int l = 0; l < NL; l++) {
         const float* W = P + t->off_layer0 + t->L.stride * l;
-        const float* LW = lora ? t->LP + t->LL.stride * l : NULL;
+        const float* LW = adapters ? t->LP + t->LL.stride * l : NULL;
         layer_act_t* a = &t->act[l];
         float* next = (l + 1 < NL) ? t->act[l + 1].layer_in : t->final_in;
         /* the input norm of every layer but the first comes out of the add that ended the previous layer */
@@ -815,7 +897,7 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
                                                   {a->xn_attn, W + t->L.v, a->v, T, kv}};
             GEMM_GROUP(qkv, 3, h, 0, 1, 0);
         }
-        if (lora) {                                                        /* the q, k and v adapters in one launch per product */
+        if (adapters) {                                                        /* the q, k and v adapters in one launch per product */
             float* outs[3] = {a->q, a->k, a->v};
             const int64_t od[3] = {qd, kv, kv};
             lora_fwd_item_t it[3];
@@ -831,13 +913,13 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
         }
         OP("attention_forward", 4.0 * D * t->attn_pairs * H, 0.0, seraph_attention_forward(a->q, a->k, a->v, a->attn_out, a->lse, starts, batch, T, H, KVH, D, scale, s));
         GEMM(a->attn_out, W + t->L.o, t->tmp_h, T, h, qd, 0, 1, 0);
-        if (lora && t->LL.A[3] >= 0 && lora_forward_add(t, a->attn_out, t->tmp_h, LW + t->LL.A[3], LW + t->LL.B[3], T, qd, h, a->xa[3])) return -1.0f;
+        if (adapters && t->LL.A[3] >= 0 && lora_forward_add(t, a->attn_out, t->tmp_h, LW + t->LL.A[3], LW + t->LL.B[3], T, qd, h, a->xa[3])) return -1.0f;
         OP("add_rmsnorm", 0.0, 16.0 * (double)(T * h), seraph_add_rmsnorm(a->layer_in, t->tmp_h, a->post_in, W + t->L.post_norm, a->xn_ffn, T, h, eps, s));
         {   /* gate and up projections (src/train.c:4718-4725) as one launch */
             const seraph_gemm_problem_t gu[2] = {{a->xn_ffn, W + t->L.gate, a->gate, T, f}, {a->xn_ffn, W + t->L.up, a->up, T, f}};
             GEMM_GROUP(gu, 2, h, 0, 1, 0);
         }
-        if (lora) {
+        if (adapters) {
             float* outs[2] = {a->gate, a->up};
             lora_fwd_item_t it[2];
             int n = 0;
@@ -847,7 +929,7 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
         }
         OP("swiglu", 0.0, 12.0 * (double)(T * f), seraph_swiglu(a->gate, a->up, a->ffn_h, (size_t)(T * f), s));
         GEMM(a->ffn_h, W + t->L.down, t->tmp_h, T, h, f, 0, 1, 0);
-        if (lora && t->LL.A[6] >= 0 && lora_forward_add(t, a->ffn_h, t->tmp_h, LW + t->LL.A[6], LW + t->LL.B[6], T, f, h, a->xa[6])) return -1.0f;
+        if (adapters && t->LL.A[6] >= 0 && lora_forward_add(t, a->ffn_h, t->tmp_h, LW + t->LL.A[6], LW + t->LL.B[6], T, f, h, a->xa[6])) return -1.0f;
         /* residual add and the norm that reads its result: the next layer's input norm, or the final norm */
         const float* next_gain = (l + 1 < NL) ? P + t->off_layer0 + t->L.stride * (l + 1) + t->L.in_norm : P + t->off_final_norm;
         float* next_xn = (l + 1 < NL) ? t->act[l + 1].xn_attn : t->xn_final;
@@ -861,10 +943,35 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
     NANCHK(t->logits, T * V, 1u);
 
     /* ---------------- loss: gradient written over the logits */
-    OP("cross_entropy_grad", 0.0, 8.0 * (double)T * (double)V + 8.0 * (double)T, seraph_cross_entropy_grad(t->logits, t->d_targets, t->logits, t->loss_rows, starts, batch, T, V, num_valid, s));
+    size_t loss_count = (size_t)T;
+    double loss_divisor = (double)num_valid;
+    const double logits_bytes = 4.0 * (double)T * (double)V;
+    if (!obj) {
+        OP("cross_entropy_grad", 0.0, 2.0 * logits_bytes + 8.0 * (double)T, seraph_cross_entropy_grad(t->logits, t->d_targets, t->logits, t->loss_rows, starts, batch, T, V, num_valid, s));
+    } else if (obj->kind == OBJ_LOGPROBS) {
+        OP("token_logprobs", 0.0, logits_bytes, seraph_token_logprobs(t->logits, t->d_targets, obj->d_logp, NULL, obj->host_entropy ? obj->d_entropy : NULL,
+                                                                      starts, batch, T, V, obj->ws, obj->ws_bytes, s));
+        CK(seraph_hip_d2h(obj->host_logp, obj->d_logp, (size_t)T * 4, s));
+        if (obj->host_entropy) CK(seraph_hip_d2h(obj->host_entropy, obj->d_entropy, (size_t)T * 4, s));
+        op_fold(t);
+        return 0.0f;
+    } else if (obj->kind == OBJ_POLICY) {
+        OP("policy_grad", 0.0, 2.0 * logits_bytes, seraph_policy_grad(t->logits, t->d_targets, obj->d_advantages, obj->d_old, obj->d_ref, obj->d_weights, t->logits,
+                                                                      t->loss_rows, NULL, NULL, NULL, obj->policy, starts, batch, T, V, num_valid,
+                                                                      obj->ws, obj->ws_bytes, s));
+    } else if (obj->kind == OBJ_PREFERENCE) {
+        OP("preference_grad", 0.0, 3.0 * logits_bytes, seraph_preference_grad(t->logits, t->d_targets, obj->d_ref, t->logits, t->loss_rows, obj->d_scores, NULL,
+                                                                              obj->preference, starts, batch / 2, T, V, obj->ws, obj->ws_bytes, s));
+        loss_count = (size_t)batch / 2;
+        loss_divisor = (double)loss_count;
+    } else {
+        OP("distill_grad", 0.0, 2.0 * logits_bytes, seraph_distill_grad(t->logits, obj->d_ids, obj->d_teacher, obj->d_teacher_lse, t->d_targets, obj->d_weights,
+                                                                        t->logits, t->loss_rows, obj->distill, starts, batch, T, V, obj->top_k, num_valid,
+                                                                        obj->ws, obj->ws_bytes, s));
+    }
     float* red_in = t->loss_rows;
     float* red_out = t->red_a;
-    for (size_t n = (size_t)T; n > 1; n = (n + 511) / 512) {                              /* src/train.c:4902-4913 */
+    for (size_t n = loss_count; n > 1; n = (n + 511) / 512) {                              /* src/train.c:4902-4913 */
         CK(seraph_reduce_sum(red_in, red_out, n, s));
         red_in = red_out;
         red_out = (red_out == t->red_a) ? t->red_b : t->red_a;
@@ -1072,25 +1179,91 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
     CK(seraph_hip_d2h(&loss_sum, red_in, sizeof(float), s));               /* waits for the whole step */
     for (int i = 0; i < 3; i++) seraph_hip_event_elapsed_ms(t->ev[i], t->ev[i + 1], &t->phase_ms[i]);
     op_fold(t);
-    return loss_sum / (float)num_valid;
+    if (!obj) return loss_sum / (float)num_valid;
+    obj->loss = (float)((double)loss_sum / loss_divisor);
+    if (obj->host_scores) CK(seraph_hip_d2h(obj->host_scores, obj->d_scores, (size_t)batch * 4, s));
+    return 0.0f;
 }
 
 float hip_train_step_full_batch(hip_trainer_t* t, const int* tokens_packed, int total_tokens,
                                 const int* seq_starts, int batch_size, int run_optimizer) {
     if (!t || t->lora) { fprintf(stderr, "ERROR: trainer is not in full-weight mode\n"); return -1.0f; }
-    return run_step(t, tokens_packed, total_tokens, seq_starts, batch_size, run_optimizer, STEP_TRAIN);
+    return run_step(t, tokens_packed, total_tokens, seq_starts, batch_size, run_optimizer, STEP_TRAIN, NULL);
 }
 
 float hip_train_step_lora_batch(hip_trainer_t* t, const int* tokens_packed, int total_tokens,
                                 const int* seq_starts, int batch_size, int run_optimizer) {
     if (!t || !t->lora) { fprintf(stderr, "ERROR: trainer is not in LoRA mode\n"); return -1.0f; }
-    return run_step(t, tokens_packed, total_tokens, seq_starts, batch_size, run_optimizer, STEP_TRAIN);
+    return run_step(t, tokens_packed, total_tokens, seq_starts, batch_size, run_optimizer, STEP_TRAIN, NULL);
 }
 
 float hip_eval_forward_batch(hip_trainer_t* t, const int* tokens_packed, int total_tokens,
                              const int* seq_starts, int batch_size) {
     if (!t) return -1.0f;
-    return run_step(t, tokens_packed, total_tokens, seq_starts, batch_size, 0, STEP_EVAL);
+    return run_step(t, tokens_packed, total_tokens, seq_starts, batch_size, 0, STEP_EVAL, NULL);
+}
+
+static int objective_step(hip_trainer_t* t, const int* tokens, int total_tokens, const int* seq_starts, int batch, int run_optimizer,
+                          objective_t* o, float* loss) {
+    if (loss) *loss = 0.0f;
+    const float r = run_step(t, tokens, total_tokens, seq_starts, batch, run_optimizer, STEP_TRAIN, o);
+    if (r == -1.0f) return -1;
+    if (loss) *loss = isnan(r) ? r : o->loss;
+    return 0;
+}
+
+int hip_token_logprobs(hip_trainer_t* t, const int* tokens_packed, int total_tokens, const int* seq_starts, int batch_size,
+                       int use_adapters, float* logp, float* entropy) {
+    if (!t || !logp) { fprintf(stderr, "ERROR: hip_token_logprobs: NULL argument\n"); return -1; }
+    for (int i = 0; i < total_tokens; i++) { logp[i] = 0.0f; if (entropy) entropy[i] = 0.0f; }
+    objective_t o = {0};
+    o.kind = OBJ_LOGPROBS;
+    o.frozen = !use_adapters;
+    o.host_logp = logp;
+    o.host_entropy = entropy;
+    return run_step(t, tokens_packed, total_tokens, seq_starts, batch_size, 0, STEP_EVAL, &o) == 0.0f ? 0 : -1;
+}
+
+int hip_train_step_policy(hip_trainer_t* t, const int* tokens_packed, int total_tokens, const int* seq_starts, int batch_size,
+                          const float* advantages, const float* old_logp, const float* ref_logp, const float* weights,
+                          const seraph_policy_options_t* options, int run_optimizer, float* loss) {
+    if (!t || !advantages || !old_logp || !options || (!ref_logp && options->kl_coef != 0.0f)) {
+        fprintf(stderr, "ERROR: hip_train_step_policy: advantages, old_logp and options are needed, and ref_logp for a KL term\n");
+        return -1;
+    }
+    objective_t o = {0};
+    o.kind = OBJ_POLICY;
+    o.advantages = advantages; o.old_logp = old_logp; o.ref_logp = ref_logp; o.weights = weights;
+    o.policy = options;
+    return objective_step(t, tokens_packed, total_tokens, seq_starts, batch_size, run_optimizer, &o, loss);
+}
+
+int hip_train_step_preference(hip_trainer_t* t, const int* tokens_packed, int total_tokens, const int* seq_starts, int pairs,
+                              const uint8_t* supervised, const float* ref_logp, const seraph_preference_options_t* options,
+                              int run_optimizer, float* loss, float* scores) {
+    if (!t || !options || !seq_starts || pairs < 1 || pairs > 0x3fffffff) {
+        fprintf(stderr, "ERROR: hip_train_step_preference: options and the offsets of 2 * pairs sequences are needed\n");
+        return -1;
+    }
+    objective_t o = {0};
+    o.kind = OBJ_PREFERENCE;
+    o.supervised = supervised; o.ref_logp = ref_logp; o.host_scores = scores;
+    o.preference = options;
+    return objective_step(t, tokens_packed, total_tokens, seq_starts, 2 * pairs, run_optimizer, &o, loss);
+}
+
+int hip_train_step_distill(hip_trainer_t* t, const int* tokens_packed, int total_tokens, const int* seq_starts, int batch_size,
+                           const uint32_t* teacher_ids, const void* teacher_logits, const float* teacher_lse, int top_k,
+                           const float* weights, const seraph_distill_options_t* options, int run_optimizer, float* loss) {
+    if (!t || !teacher_ids || !teacher_logits || !options || top_k < 1 || top_k > 1024) {
+        fprintf(stderr, "ERROR: hip_train_step_distill: a teacher's list of 1 to 1024 logits per token and options are needed\n");
+        return -1;
+    }
+    objective_t o = {0};
+    o.kind = OBJ_DISTILL;
+    o.teacher_ids = teacher_ids; o.teacher_logits = teacher_logits; o.teacher_lse = teacher_lse; o.top_k = top_k; o.weights = weights;
+    o.distill = options;
+    return objective_step(t, tokens_packed, total_tokens, seq_starts, batch_size, run_optimizer, &o, loss);
 }
 
 /* src/train_cuda.c:2812-2847 */

@@ -6,7 +6,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import SeraphError, backend
+from ._lib import DistillOptions, PolicyOptions, PreferenceOptions, SeraphError, backend
 
 
 class ModelConfig(C.Structure):
@@ -95,6 +95,11 @@ def _lib():
         lib.hip_trainer_nan_flags.argtypes = [C.c_void_p, C.c_void_p, C.c_int]
         lib.hip_param_layout.argtypes = [C.POINTER(ModelConfig), C.POINTER(ParamLayout)]
         lib.hip_lora_layout.argtypes = [C.POINTER(ModelConfig), C.POINTER(LoraLayout)]
+        p, i, out = C.c_void_p, C.c_int, C.POINTER(C.c_float)
+        lib.hip_token_logprobs.argtypes = [p, p, i, p, i, i, p, p]
+        lib.hip_train_step_policy.argtypes = [p, p, i, p, i, p, p, p, p, C.POINTER(PolicyOptions), i, out]
+        lib.hip_train_step_preference.argtypes = [p, p, i, p, i, p, p, C.POINTER(PreferenceOptions), i, out, p]
+        lib.hip_train_step_distill.argtypes = [p, p, i, p, i, p, p, p, i, p, C.POINTER(DistillOptions), i, out]
         lib._seraph_train_bound = True
     return lib
 
@@ -166,6 +171,82 @@ class Trainer:
         if loss < 0:
             raise SeraphError("training step failed (see stderr)")
         return float(loss)
+
+    @staticmethod
+    def _batch(tokens, seq_starts):
+        """(tokens, their address and number, the offsets' address, the sequences, what has to stay alive)"""
+        tokens = np.ascontiguousarray(tokens, np.int32)
+        if seq_starts is None:
+            return tokens.ctypes.data, tokens.size, None, 1, (tokens,)
+        seq_starts = np.ascontiguousarray(seq_starts, np.int32)
+        return tokens.ctypes.data, tokens.size, seq_starts.ctypes.data, seq_starts.size - 1, (tokens, seq_starts)
+
+    @staticmethod
+    def _rows(name, a, total, dtype=np.float32, cols=None):
+        """An array per token as the library reads it; None for None."""
+        if a is None:
+            return None
+        a = np.ascontiguousarray(a, dtype)
+        if a.shape != ((total,) if cols is None else (total, cols)):
+            raise SeraphError(f"{name} has the shape {a.shape}; one entry for each of {total} tokens is needed")
+        return a
+
+    def token_logprobs(self, tokens, seq_starts=None, adapters=True, want_entropy=False):
+        """Log-probability of each token's successor within its sequence (0 for the last one), and on request the entropy
+        of each prediction.  Forward only; adapters=False: the frozen base model of a LoRA trainer."""
+        tp, total, sp, batch, keep = self._batch(tokens, seq_starts)
+        logp = np.zeros(total, np.float32)
+        entropy = np.zeros(total, np.float32) if want_entropy else None
+        if _lib().hip_token_logprobs(self._h, tp, total, sp, batch, 1 if adapters else 0, logp.ctypes.data,
+                                     None if entropy is None else entropy.ctypes.data) != 0:
+            raise SeraphError("token_logprobs failed (see stderr)")
+        return (logp, entropy) if want_entropy else logp
+
+    def step_policy(self, tokens, seq_starts, advantages, old_logp, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_coef=0.0,
+                    entropy_coef=0.0, run_optimizer=True):
+        """A step on the clipped policy loss (ops.policy_grad); arrays per token as in hip_train.h, weights 0 for prompts."""
+        tp, total, sp, batch, keep = self._batch(tokens, seq_starts)
+        rows = [self._rows(n, a, total) for n, a in (("advantages", advantages), ("old_logp", old_logp), ("ref_logp", ref_logp), ("weights", weights))]
+        loss = C.c_float()
+        if _lib().hip_train_step_policy(self._h, tp, total, sp, batch, *[None if a is None else a.ctypes.data for a in rows],
+                                        PolicyOptions(clip[0], clip[1], kl_coef, entropy_coef), 1 if run_optimizer else 0, C.byref(loss)) != 0:
+            raise SeraphError("policy step failed (see stderr)")
+        return float(loss.value)
+
+    def step_preference(self, tokens, seq_starts, supervised=None, ref_logp=None, kind="sigmoid", beta=0.1, label_smoothing=0.0, margin=0.0,
+                        average=False, run_optimizer=True):
+        """A step on the preference loss of pairs of sequences (2i chosen, 2i + 1 rejected): (mean loss, score of each sequence)."""
+        from .ops import PREFERENCE_KINDS
+        tp, total, sp, batch, keep = self._batch(tokens, seq_starts)
+        if sp is None or batch % 2 or kind not in PREFERENCE_KINDS:
+            raise SeraphError(f"a preference step needs the offsets of pairs of sequences and one of {sorted(PREFERENCE_KINDS)}")
+        mask = None if supervised is None else self._rows("supervised", np.asarray(supervised) != 0, total, np.uint8)
+        ref = self._rows("ref_logp", ref_logp, total)
+        loss, scores = C.c_float(), np.zeros(batch, np.float32)
+        if _lib().hip_train_step_preference(self._h, tp, total, sp, batch // 2, None if mask is None else mask.ctypes.data,
+                                            None if ref is None else ref.ctypes.data,
+                                            PreferenceOptions(PREFERENCE_KINDS[kind], beta, label_smoothing, margin, 1 if average else 0),
+                                            1 if run_optimizer else 0, C.byref(loss), scores.ctypes.data) != 0:
+            raise SeraphError("preference step failed (see stderr)")
+        return float(loss.value), scores
+
+    def step_distill(self, tokens, seq_starts, teacher_ids, teacher_logits, teacher_lse=None, weights=None, temperature=1.0, soft_coef=1.0,
+                     hard_coef=0.0, run_optimizer=True):
+        """A step on distillation from a teacher's listed logits [tokens, top_k] (float32 or float16 arrays)."""
+        tp, total, sp, batch, keep = self._batch(tokens, seq_starts)
+        teacher_logits = np.asarray(teacher_logits)
+        half = teacher_logits.dtype == np.float16
+        top_k = teacher_logits.shape[1] if teacher_logits.ndim == 2 else 0
+        ids = self._rows("teacher_ids", teacher_ids, total, np.uint32, top_k)
+        listed = self._rows("teacher_logits", teacher_logits, total, np.float16 if half else np.float32, top_k)
+        lse, w = self._rows("teacher_lse", teacher_lse, total), self._rows("weights", weights, total)
+        loss = C.c_float()
+        if _lib().hip_train_step_distill(self._h, tp, total, sp, batch, ids.ctypes.data, listed.ctypes.data, None if lse is None else lse.ctypes.data,
+                                         top_k, None if w is None else w.ctypes.data,
+                                         DistillOptions(temperature, soft_coef, hard_coef, 1 if half else 0), 1 if run_optimizer else 0,
+                                         C.byref(loss)) != 0:
+            raise SeraphError("distillation step failed (see stderr)")
+        return float(loss.value)
 
     def eval_forward(self, tokens, seq_starts=None):
         """Forward and loss only (cuda_eval_forward of the reference); changes no state."""
