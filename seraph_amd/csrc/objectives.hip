@@ -162,15 +162,15 @@ struct DistillOp {
 };
 
 // ---------------------------------------------------------------- a teacher's list
-// Turns a row's list into the mass q of each entry, its logits z, and the row's sums.  One wave's work: the others of its
-// workgroup go on with the row, and meet the list again behind a barrier.  The logits are gathered before anything of
-// the row is overwritten.
+// A row's list becomes the mass q of each entry, its logits z, gathered before anything of the row is overwritten, and the
+// row's sums.  The entries are chained in buckets, so an id listed twice meets itself in its chain.  That is rare, and
+// only then are all pairs compared, to add up an id's mass in list order.
 //
-// The entries are chained in buckets.  Where the workgroup holds the whole row (HELD) a bucket is a vector of it, so the
-// lane that is about to store a vector finds the entries in it by one look; elsewhere it is a hash of the id.  Either
-// way an id listed twice meets itself in its chain.  That is rare, and only then are all pairs compared: each entry of such an
-// id takes the id's whole mass, added in list order (HELD: the first does and the others take none, so that the
-// order of a chain, which is the order of atomics, changes nothing).
+// Where a workgroup holds a whole row (HELD) all of its waves share the list's work, between the barriers that the row needs
+// anyway, and a bucket is a vector of the row: the lane that is about to store a vector finds the entries in it by
+// one look.  Of an id listed twice the first entry then takes the whole mass and the others none, so that the order of
+// a chain, which is the order of atomics, changes nothing.  Elsewhere one wave does the work, a bucket is a hash of the id,
+// and every entry of an id holds the whole mass, so whichever is used last leaves the same value.
 //
 // The list's LDS is sized by the call: with room for the longest list always, short ones would cost the wave of
 // prepare_rows_kernel most of its occupancy.
@@ -192,12 +192,41 @@ __device__ __forceinline__ ListRoom list_room(void* lds, int top_k, int buckets)
 }
 constexpr uint32_t kNoId = 0xffffffffu;
 
-// HELD: 0 the single values ahead of the vectors, 1 + i vector i, 1 + n4 those behind
-template <bool HELD>
-__device__ __forceinline__ int list_bucket(const ListRoom& room, const RowShape& sh, uint32_t id) {
-    if (!HELD) return (int)((id * 2654435761u) >> 8 & (uint32_t)(room.buckets - 1));
+// 0: the single values ahead of the vectors, 1 + i: vector i, 1 + n4: those behind
+__device__ __forceinline__ int held_bucket(const RowShape& sh, uint32_t id) {
     const int i4 = ((int)id - sh.head) >> 2;
     return (int)id < sh.head ? 0 : i4 < sh.n4 ? 1 + i4 : 1 + sh.n4;
+}
+__device__ __forceinline__ int hashed_bucket(const ListRoom& room, uint32_t id) { return (int)((id * 2654435761u) >> 8 & (uint32_t)(room.buckets - 1)); }
+
+__device__ __forceinline__ bool meets_itself(const ListRoom& room, int i, int bucket) {
+    bool twice = false;
+    for (uint32_t o = room.first[bucket]; o; o = room.next[o - 1]) twice |= o != (uint32_t)i + 1u && room.id[o - 1] == room.id[i];
+    return twice;
+}
+// the mass of entry i's id; `first`: none where an earlier entry has it
+__device__ __forceinline__ float mass_of_id(const ListRoom& room, int n, int i, bool first) {
+    float sum = 0.0f;
+    for (int o = 0; o < n; o++)
+        if (room.id[o] == room.id[i]) {
+            if (first && o < i) return 0.0f;
+            sum += room.q[o];
+        }
+    return sum;
+}
+
+// log q_i = (u_i - m) / T + log; q sums up to s exp(log), which is 1 where the list is the whole distribution
+struct ListNorm { double log; float factor; double mass; };
+__device__ __forceinline__ ListNorm list_norm(const TeacherList& l, int64_t r, float m, float s, double inv_temp) {
+    ListNorm o;
+    o.log = l.lse ? (double)m * inv_temp - (double)l.lse[r] : -log_of(s);
+    o.factor = l.lse ? exp_of((float)o.log, 0.0f, kUnitScale) : 1.0f / s;
+    o.mass = s == 0.0f ? 0.0 : l.lse ? (double)s * (double)o.factor : s == s ? 1.0 : (double)s;      // (no entry at all: no mass, not NaN)
+    return o;
+}
+// what an entry of mass p adds to the sum q (log q - (z - at) / T)
+__device__ __forceinline__ double cross_part(float p, float u, float m, float z, float at, double inv_temp, double log_norm) {
+    return p == 0.0f ? 0.0 : (double)p * (((double)u - (double)m) * inv_temp + log_norm - ((double)z - (double)at) * inv_temp);
 }
 
 __device__ __forceinline__ void wave_sync() {                     // the wave's own LDS writes are complete and in order
@@ -205,9 +234,8 @@ __device__ __forceinline__ void wave_sync() {                     // the wave's 
     __builtin_amdgcn_wave_barrier();
 }
 
-template <bool HELD>
-__device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, const float* row, const RowShape& sh, int64_t cols, double inv_temp, ExpScale k,
-                                              const ListRoom& room) {
+// One wave's form.
+__device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, const float* row, int64_t cols, double inv_temp, ExpScale k, const ListRoom& room) {
     const int lane = (int)threadIdx.x & 63, n = l.top_k;
     const int64_t base = r * n;
     float m = kLowest, at = kLowest;
@@ -236,7 +264,7 @@ __device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, c
             room.q[i] = u[j];
             room.z[i] = z[j];
             if (id[j] != kNoId) {
-                room.next[i] = atomicExch(&room.first[list_bucket<HELD>(room, sh, id[j])], (uint32_t)i + 1u);
+                room.next[i] = atomicExch(&room.first[hashed_bucket(room, id[j])], (uint32_t)i + 1u);
                 m = fmaxf(m, u[j]);
                 at = fmaxf(at, z[j]);
             }
@@ -244,11 +272,8 @@ __device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, c
     }
     wave_sync();
     bool twice = false;
-    for (int i = lane; i < n; i += 64) {
-        const uint32_t id = room.id[i];
-        if (id == kNoId) continue;
-        for (uint32_t o = room.first[list_bucket<HELD>(room, sh, id)]; o; o = room.next[o - 1]) twice |= o != (uint32_t)i + 1u && room.id[o - 1] == id;
-    }
+    for (int i = lane; i < n; i += 64)
+        if (room.id[i] != kNoId) twice |= meets_itself(room, i, hashed_bucket(room, room.id[i]));
     twice = __any(twice);
     m = wave_top(m);
     at = wave_top(at);
@@ -256,17 +281,11 @@ __device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, c
     for (int i = lane; i < n; i += 64)
         if (room.id[i] != kNoId) s += exp_of(room.q[i], m, k);
     s = wave_total(s);
-    // log q_i = (u_i - m) / T + log_norm; q sums up to s exp(log_norm), which is 1 where the list is the whole distribution
-    const double log_norm = l.lse ? (double)m * inv_temp - (double)l.lse[r] : -log_of(s);
-    const float norm = l.lse ? exp_of((float)log_norm, 0.0f, kUnitScale) : 1.0f / s;
+    const ListNorm norm = list_norm(l, r, m, s, inv_temp);
     double cross = 0.0;
     for (int i = lane; i < n; i += 64) {
-        float p = 0.0f;
-        if (room.id[i] != kNoId && s != 0.0f) {                   // (no entry at all: no mass, not NaN)
-            const float u = room.q[i];
-            p = exp_of(u, m, k) * norm;
-            if (p != 0.0f) cross += (double)p * (((double)u - (double)m) * inv_temp + log_norm - ((double)room.z[i] - (double)at) * inv_temp);
-        }
+        const float u = room.q[i], p = room.id[i] != kNoId && s != 0.0f ? exp_of(u, m, k) * norm.factor : 0.0f;
+        cross += cross_part(p, u, m, room.z[i], at, inv_temp, norm.log);
         room.q[i] = p;
     }
     cross = wave_total(cross);
@@ -274,26 +293,14 @@ __device__ __forceinline__ ListSums read_list(const TeacherList& l, int64_t r, c
         wave_sync();
         float part[kMaxTopK / 64];
 #pragma unroll
-        for (int j = 0; j < kMaxTopK / 64; j++) {
-            const int i = lane + j * 64;
-            part[j] = 0.0f;
-            if (i < n) {
-                bool earlier = false;
-                for (int o = 0; o < n; o++)
-                    if (room.id[o] == room.id[i]) {
-                        part[j] += room.q[o];
-                        earlier |= o < i;
-                    }
-                if (HELD && earlier) part[j] = 0.0f;
-            }
-        }
+        for (int j = 0; j < kMaxTopK / 64; j++) part[j] = lane + j * 64 < n ? mass_of_id(room, n, lane + j * 64, false) : 0.0f;
         wave_sync();
 #pragma unroll
         for (int j = 0; j < kMaxTopK / 64; j++)
             if (lane + j * 64 < n) room.q[lane + j * 64] = part[j];
     }
     wave_sync();
-    return ListSums{s == 0.0f ? 0.0 : l.lse ? (double)s * (double)norm : s == s ? 1.0 : (double)s, cross, at};
+    return ListSums{norm.mass, cross, at};
 }
 
 // ---------------------------------------------------------------- rows held in registers
@@ -306,6 +313,9 @@ template <class Op, int EXTRA, int BLOCK, int VPT>
 __global__ __launch_bounds__(BLOCK, held_waves(VPT, Op::kList)) void held_rows_kernel(Op op, const float* logits, float* grad, int cols) {
     __shared__ float red[3][BLOCK / 64];
     __shared__ RowGrad bcast;
+    __shared__ float list_red[3][BLOCK / 64];
+    __shared__ double list_cross[BLOCK / 64];
+    __shared__ int listed_twice;
     extern __shared__ char list_lds[];
     const int64_t row = blockIdx.x;
     const float* x = logits + row * cols;
@@ -323,6 +333,22 @@ __global__ __launch_bounds__(BLOCK, held_waves(VPT, Op::kList)) void held_rows_k
         if (threadIdx.x == 0) op.dead(row);
         return;
     }
+    // a list's ids and logits are asked for ahead of the row, and the row's logits at its ids behind it: memory answers in order
+    constexpr int kEntries = kMaxTopK / BLOCK;
+    uint32_t id[Op::kList ? kEntries : 1];
+    float u[Op::kList ? kEntries : 1];
+    ListRoom room{};
+    if constexpr (Op::kList) {
+        room = list_room(list_lds, op.list.top_k, sh.n4 + 2);
+#pragma unroll
+        for (int j = 0; j < kEntries; j++) {
+            const int i = j * BLOCK + (int)threadIdx.x;
+            id[j] = i < op.list.top_k ? op.list.ids[row * op.list.top_k + i] : kNoId;
+            u[j] = i < op.list.top_k ? op.list.logit(row * op.list.top_k + i) : 0.0f;
+        }
+        for (int i = threadIdx.x; i < room.buckets; i += BLOCK) room.first[i] = 0u;
+        if (threadIdx.x == 0) listed_twice = 0;
+    }
     f4 v[VPT];
 #pragma unroll
     for (int k = 0; k < VPT; k++) v[k] = xs.load<kNontemporal>((k * BLOCK + (int)threadIdx.x) * 16);
@@ -332,11 +358,28 @@ __global__ __launch_bounds__(BLOCK, held_waves(VPT, Op::kList)) void held_rows_k
         const int64_t t = op.target(row);
         if (t >= 0) zt = x[t];
     }
-    ListRoom room{};
-    ListSums sums{0.0, 0.0, 0.0f};
+    float lm = kLowest, at = kLowest;
     if constexpr (Op::kList) {
-        room = list_room(list_lds, op.list.top_k, sh.n4 + 2);
-        if (threadIdx.x < 64) sums = read_list<true>(op.list, row, x, sh, cols, op.inv_temp, op.k, room);
+#pragma unroll
+        for (int j = 0; j < kEntries; j++) {
+            const int i = j * BLOCK + (int)threadIdx.x;
+            if (i >= op.list.top_k) break;
+            if ((int64_t)id[j] >= cols) id[j] = kNoId;
+            room.id[i] = id[j];
+            room.q[i] = u[j];
+            if (id[j] != kNoId) {
+                const float z = x[id[j]];
+                room.z[i] = z;
+                lm = fmaxf(lm, u[j]);
+                at = fmaxf(at, z);
+            }
+        }
+        lm = wave_top(lm);
+        at = wave_top(at);
+        if ((threadIdx.x & 63) == 0) {
+            list_red[0][threadIdx.x >> 6] = lm;
+            list_red[1][threadIdx.x >> 6] = at;
+        }
     }
     const ExpScale ks = op.k;
     float m = fmaxf(kLowest, one);
@@ -346,6 +389,18 @@ __global__ __launch_bounds__(BLOCK, held_waves(VPT, Op::kList)) void held_rows_k
         m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
     }
     m = block_max<BLOCK>(m, red[0]);
+    if constexpr (Op::kList) {                                    // the buckets are clear, the list's maxima complete
+#pragma unroll
+        for (int w = 0; w < BLOCK / 64; w++) { lm = fmaxf(lm, list_red[0][w]); at = fmaxf(at, list_red[1][w]); }
+        float part = 0.0f;
+        for (int i = threadIdx.x; i < op.list.top_k; i += BLOCK)
+            if (room.id[i] != kNoId) {
+                room.next[i] = atomicExch(&room.first[held_bucket(sh, room.id[i])], (uint32_t)i + 1u);
+                part += exp_of(room.q[i], lm, ks);
+            }
+        part = wave_total(part);
+        if ((threadIdx.x & 63) == 0) list_red[2][threadIdx.x >> 6] = part;
+    }
     float e1 = exp_of(one, m, ks), s = e1, ex = EXTRA != kNone ? extra_of<EXTRA>(one, m, e1) : 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
@@ -360,9 +415,51 @@ __global__ __launch_bounds__(BLOCK, held_waves(VPT, Op::kList)) void held_rows_k
     }
     if (EXTRA != kNone) block_sum2<BLOCK>(s, ex, red[1]);
     else s = block_sum<BLOCK>(s, red[1]);
-    if (threadIdx.x == 0) bcast = op.template finish<EXTRA>(row, RowStats{m, s, ex}, zt, sums);
-    if constexpr (Op::kGrad) {
+    const RowStats stats{m, s, ex};
+    ListSums sums{0.0, 0.0, at};
+    if constexpr (Op::kList) {                                    // the chains and the list's sum are complete
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < BLOCK / 64; w++) total += list_red[2][w];
+        const ListNorm norm = list_norm(op.list, row, lm, total, op.inv_temp);
+        sums.mass = norm.mass;
+        double cross = 0.0;
+        bool twice = false;
+        for (int i = threadIdx.x; i < op.list.top_k; i += BLOCK) {
+            float p = 0.0f;
+            if (room.id[i] != kNoId) {
+                p = total != 0.0f ? exp_of(room.q[i], lm, ks) * norm.factor : 0.0f;
+                cross += cross_part(p, room.q[i], lm, room.z[i], at, op.inv_temp, norm.log);
+                twice |= meets_itself(room, i, held_bucket(sh, room.id[i]));
+            }
+            room.q[i] = p;
+        }
+        cross = wave_total(cross);
+        if ((threadIdx.x & 63) == 0) list_cross[threadIdx.x >> 6] = cross;
+        if (__any(twice) && (threadIdx.x & 63) == 0) listed_twice = 1;
+    }
+    if (threadIdx.x == 0) bcast = op.template finish<EXTRA>(row, stats, zt, sums, !Op::kList);
+    if constexpr (Op::kList) {
         __syncthreads();
+        if (threadIdx.x == 0) {                                   // the loss is the one thing that needs the last sum
+            for (int w = 0; w < BLOCK / 64; w++) sums.cross += list_cross[w];
+            op.template finish<EXTRA>(row, stats, zt, sums, true);
+        }
+        if (listed_twice) {                                       // (the same for the whole workgroup)
+            float part[kEntries];
+#pragma unroll
+            for (int j = 0; j < kEntries; j++) {
+                const int i = j * BLOCK + (int)threadIdx.x;
+                part[j] = i < op.list.top_k ? mass_of_id(room, op.list.top_k, i, true) : 0.0f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < kEntries; j++)
+                if (j * BLOCK + (int)threadIdx.x < op.list.top_k) room.q[j * BLOCK + (int)threadIdx.x] = part[j];
+        }
+    }
+    if constexpr (Op::kGrad) {
+        if (!Op::kList || listed_twice) __syncthreads();
         const RowGrad g = bcast;
         const SlotBuffer gs(out + sh.head, sh.n4);
         float es = 0.0f;
@@ -468,7 +565,7 @@ __global__ __launch_bounds__(64) void prepare_rows_kernel(Op op, const float* lo
         const float* x = logits + row * cols;
         const bool live = op.live(row);
         if (live) {
-            sums = read_list<false>(op.list, row, x, RowShape(x, cols), cols, op.inv_temp, op.k, room);
+            sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
             for (int i = threadIdx.x; i < op.list.top_k; i += 64) {
                 list_q[row * op.list.top_k + i] = room.q[i];
                 list_z[row * op.list.top_k + i] = room.z[i];
@@ -897,7 +994,7 @@ __global__ __launch_bounds__(kBlock) void swept_rows_kernel(Op op, const float* 
     ListSums sums{0.0, 0.0, 0.0f};
     if constexpr (Op::kList) {
         room = list_room(list_lds, op.list.top_k, hash_buckets(op.list.top_k));
-        if (threadIdx.x < 64) sums = read_list<false>(op.list, row, x, RowShape(x, cols), cols, op.inv_temp, op.k, room);
+        if (threadIdx.x < 64) sums = read_list(op.list, row, x, cols, op.inv_temp, op.k, room);
     }
     if (threadIdx.x == 0) {
         const int64_t t = op.target(row);
@@ -980,7 +1077,7 @@ struct PairRowsOp {
         if (logp_rows) logp_rows[r] = 0.0f;
     }
     template <int EXTRA>
-    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&) const {
+    __device__ __forceinline__ RowGrad finish(int64_t r, RowStats st, float zt, const ListSums&, bool = true) const {
         runs[r] = RowStats{st.m, st.s, zt};
         return RowGrad{0.0f, 0.0f, 0.0f, -1};
     }
