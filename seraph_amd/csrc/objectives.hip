@@ -22,11 +22,15 @@ struct RowGrad { float a, b, c; int64_t target; };
 
 template <int EXTRA>
 __device__ __forceinline__ float grad_at(float z, float m, ExpScale k, const RowGrad& g) {
-    const float e = exp_of(z, m, k);
+    const float e = exp_once(z, m, k);
     if (EXTRA == kEntropy) return e == 0.0f ? e * g.a : e * (g.a + g.b * (z - m));
-    if (EXTRA == kSecond) return g.a * e + g.b * exp_of(z, m, kUnitScale);
+    if (EXTRA == kSecond) return g.a * e + g.b * exp_once(z, m, kUnitScale);
+    if (EXTRA == kSquare) return e * (g.a + g.b * e);
     return g.a * e;
 }
+// the same from the exponential
+template <int EXTRA>
+__device__ __forceinline__ float grad_of_exp(float e, float a, float b) { return EXTRA == kSquare ? e * (a + b * e) : a * e; }
 
 // ---------------------------------------------------------------- the objectives
 // An objective is a struct of its arguments.  dead(): the outputs of a row that is not supervised.  finish(): called by one lane
@@ -150,11 +154,11 @@ struct DistillOp {
             g.a = soft_coef * (float)inv_temp * sc * mass / st.s;
         }
         if (g.target >= 0) {
-            const float s1 = EXTRA == kSecond ? st.x : st.s;      // the sum at T = 1
+            const float s1 = EXTRA == kNone ? st.s : st.x;      // the sum at T = 1
             loss += (double)hard_coef * (log_of(s1) - ((double)zt - (double)st.m));
             g.c = hard_coef * sc;
-            if (EXTRA == kSecond) g.b = g.c / s1;
-            else g.a += g.c / s1;
+            if (EXTRA == kNone) g.a += g.c / s1;
+            else g.b = g.c / s1;
         }
         if (writes) loss_rows[r] = (float)((double)w * loss);
         return g;
@@ -409,7 +413,7 @@ __global__ __launch_bounds__(BLOCK, held_waves(VPT, Op::kList)) void held_rows_k
             const float e = exp_of(v[k][c], m, ks);
             s += e;
             if (EXTRA != kNone) ex += extra_of<EXTRA>(v[k][c], m, e);
-            else if (Op::kGrad) v[k][c] = e;                      // the gradient is a multiple of it
+            if (Op::kGrad && holds_exp(EXTRA)) v[k][c] = e;
         }
         if (!Op::kList) asm volatile("" : "+v"(v[k]));            // four values stay the four registers that a store takes
     }
@@ -466,14 +470,13 @@ __global__ __launch_bounds__(BLOCK, held_waves(VPT, Op::kList)) void held_rows_k
         if constexpr (Op::kList) es = op.entry_scale(row);
         const int tv = (int)g.target - sh.head, t4 = g.target >= sh.head ? tv >> 2 : -1;      // the target's place among the vectors
         const f4 off_target = {(tv & 3) == 0 ? g.c : 0.0f, (tv & 3) == 1 ? g.c : 0.0f, (tv & 3) == 2 ? g.c : 0.0f, (tv & 3) == 3 ? g.c : 0.0f};
-        // the exponentials are formed again from the logits: kept from the sums they would double the registers of a row
-        if (EXTRA != kNone) asm volatile("" : "+v"(m));
+        if (!holds_exp(EXTRA)) asm volatile("" : "+v"(m));        // the sums' exponentials are not to be kept for here
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
             const int i4 = k * BLOCK + (int)threadIdx.x;
             f4 r;
 #pragma unroll
-            for (int c = 0; c < 4; c++) r[c] = EXTRA == kNone ? g.a * v[k][c] : grad_at<EXTRA>(v[k][c], m, ks, g);
+            for (int c = 0; c < 4; c++) r[c] = holds_exp(EXTRA) ? grad_of_exp<EXTRA>(v[k][c], g.a, g.b) : grad_at<EXTRA>(v[k][c], m, ks, g);
             if (t4 == i4) r -= off_target;
             if constexpr (Op::kList) {
                 for (uint32_t o = i4 < sh.n4 ? room.first[1 + i4] : 0u; o; o = room.next[o - 1]) {
@@ -542,7 +545,7 @@ __device__ __forceinline__ RowStats against(RowStats st, float m, ExpScale k) {
     const float r = exp_of(st.m, m, k);
     RowStats o{m, st.s == 0.0f ? 0.0f : st.s * r, 0.0f};
     if (EXTRA == kEntropy) o.x = st.s == 0.0f || r == 0.0f ? 0.0f : (st.x + (st.m - m) * st.s) * r;
-    if (EXTRA == kSecond) o.x = st.x == 0.0f ? 0.0f : st.x * exp_of(st.m, m, kUnitScale);
+    if (EXTRA == kSecond || EXTRA == kSquare) o.x = st.x == 0.0f ? 0.0f : st.x * exp_of(st.m, m, kUnitScale);
     return o;
 }
 
@@ -674,7 +677,7 @@ __global__ __launch_bounds__(kBlock, kPartsPerCu) void shared_rows_kernel(Op op,
                 const float e = exp_of(v[k][c], mine.m, ks);
                 s += e;
                 if (EXTRA != kNone) ex += extra_of<EXTRA>(v[k][c], mine.m, e);
-                else v[k][c] = e;
+                if (holds_exp(EXTRA)) v[k][c] = e;
             }
             asm volatile("" : "+v"(v[k]));                        // four exponentials stay the four registers that a store takes
         }
@@ -765,8 +768,9 @@ __global__ __launch_bounds__(kBlock, kPartsPerCu) void shared_rows_kernel(Op op,
         }
         const RowGrad g = bcast.g;
         float rm = bcast.st.m;
-        if (EXTRA != kNone) asm volatile("" : "+v"(rm));          // form the exponentials again rather than keep both
-        const float back = EXTRA == kNone ? g.a * exp_of(mine.m, rm, ks) : 0.0f;
+        if (!holds_exp(EXTRA)) asm volatile("" : "+v"(rm));       // the sums' exponentials are not to be kept for here
+        const float up = holds_exp(EXTRA) ? exp_of(mine.m, rm, ks) : 0.0f;      // this part's exponentials against the row's maximum
+        const float ga = g.a * up, gb = g.b * up * up;
         const int tv = (int)g.target - sh.head, target_bytes = g.target >= sh.head ? (tv >> 2) * 16 : -1;
         const f4 off_target = {(tv & 3) == 0 ? g.c : 0.0f, (tv & 3) == 1 ? g.c : 0.0f, (tv & 3) == 2 ? g.c : 0.0f, (tv & 3) == 3 ? g.c : 0.0f};
         const int64_t single = part == 0 ? sh.single((int)threadIdx.x) : -1;
@@ -783,7 +787,7 @@ __global__ __launch_bounds__(kBlock, kPartsPerCu) void shared_rows_kernel(Op op,
         for (int k = 0; k < kPartVpt; k++) {
             f4 r;
 #pragma unroll
-            for (int c = 0; c < 4; c++) r[c] = EXTRA == kNone ? back * v[k][c] : grad_at<EXTRA>(v[k][c], rm, ks, g);
+            for (int c = 0; c < 4; c++) r[c] = holds_exp(EXTRA) ? grad_of_exp<EXTRA>(v[k][c], ga, gb) : grad_at<EXTRA>(v[k][c], rm, ks, g);
             if (target_bytes == off) r -= off_target;
             gs.store<kNontemporal>(r, off);
             v[k] = xs.load<kNontemporal>(off);
@@ -1353,7 +1357,8 @@ int seraph_distill_grad(const float* logits, const uint32_t* teacher_ids, const 
     const float scale = valid_rows > 0 ? 1.0f / (float)valid_rows : 0.0f;
     DistillOp op{{nullptr, weights, seq_starts, batch, cols}, {teacher_ids, teacher_logits, teacher_lse, options->teacher_type, (int)top_k},
                  targets, loss_rows, options->soft_coef, options->hard_coef, scale, ExpScale::of(1.0 / (double)options->temperature), 1.0 / (double)options->temperature};
-    // at T = 1 the two parts share their exponentials
+    // at T = 1 the two parts share their exponentials, at T = 2 one is the other's square
+    if (options->hard_coef != 0.0f && options->temperature == 2.0f) return launch_rows<DistillOp, kSquare>(op, logits, grad, rows, cols, top_k, ws, as_stream(s));
     if (options->hard_coef != 0.0f && options->temperature != 1.0f) return launch_rows<DistillOp, kSecond>(op, logits, grad, rows, cols, top_k, ws, as_stream(s));
     return launch_rows<DistillOp, kNone>(op, logits, grad, rows, cols, top_k, ws, as_stream(s));
 }

@@ -21,8 +21,12 @@ typedef float f4a4 __attribute__((ext_vector_type(4), aligned(4)));      // 16 b
 enum Extra {
     kNone,        // nothing
     kEntropy,     // the sum of exp(z - m) (z - m)      (T = 1)
-    kSecond       // the sum of exp(z - m), beside the one at T
+    kSecond,      // the sum of exp(z - m), beside the one at T
+    kSquare       // the same at T = 2, where it is the square of the first
 };
+// Whether the gradient follows from the exponential alone, which then takes the logit's register; else it is formed again
+// from the logit, rather than kept beside it.
+constexpr bool holds_exp(int extra) { return extra == kNone || extra == kSquare; }
 
 struct RowStats { float m, s, x; };
 
@@ -46,6 +50,9 @@ __device__ __forceinline__ float exp_of(float z, float m, ExpScale k) {
     const float d = z - m;
     return __builtin_amdgcn_exp2f(fmaf(d, k.hi, d * k.lo));
 }
+
+// The same for the gradient, where nothing adds up over tokens: the first part of the factor alone.
+__device__ __forceinline__ float exp_once(float z, float m, ExpScale k) { return __builtin_amdgcn_exp2f((z - m) * k.hi); }
 
 // log s in 64 bits, off by 1e-7 at most: the exponent is exact, the logarithm of the mantissa lies in [-ln 2, 0].  A few
 // instructions and registers, where log(double) needs dozens of both beside a row that fills a lane's registers.
@@ -73,6 +80,7 @@ template <int EXTRA>
 __device__ __forceinline__ float extra_of(float z, float m, float e) {
     if (EXTRA == kEntropy) return e > 0.0f ? e * (z - m) : (e == 0.0f ? 0.0f : e);      // exp(-inf) (-inf) counts 0, NaN stays
     if (EXTRA == kSecond) return exp_of(z, m, kUnitScale);
+    if (EXTRA == kSquare) return e * e;
     return 0.0f;
 }
 

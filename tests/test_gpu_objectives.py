@@ -166,7 +166,8 @@ def run_distill(ops, z, ids, teacher, valid, in_place=False, shift=0, **kw):
 
 
 @pytest.mark.parametrize("cols", COLS)
-@pytest.mark.parametrize("top_k,dtype,temperature,hard", [(1, "float32", 1.0, 0.0), (7, "bfloat16", 2.0, 0.3), (64, "float16", 1.0, 0.3), (300, "float32", 0.5, 0.0)])
+@pytest.mark.parametrize("top_k,dtype,temperature,hard", [(1, "float32", 1.0, 0.0), (7, "bfloat16", 2.0, 0.3), (64, "float16", 1.0, 0.3), (300, "float32", 0.5, 0.0),
+                                                         (33, "bfloat16", 0.7, 0.3), (20, "float16", 3.0, 0.5)])
 def test_distill(ops, cols, top_k, dtype, temperature, hard):
     rows = 6
     r, z, t = make(rows, cols, cols + 3)
@@ -285,7 +286,7 @@ def test_masked_logits_inside_a_row(ops, cols):
     teacher[(2, 3, 7, 10), :] = -float("inf")                     # mass only where the student can follow
     for i in (2, 3, 7, 10):
         teacher[i, int(t[i])] = 1.0
-    for temperature, hard in ((1.0, 0.0), (2.0, 0.5)):
+    for temperature, hard in ((1.0, 0.0), (2.0, 0.5), (1.7, 0.5)):
         want = ref.distill(z, ids, teacher.numpy(), rows, temperature=temperature, hard=hard, targets=t)
         compare(run_distill(ops, z, ids, teacher, rows, temperature=temperature, hard_coef=hard, targets=t), want, f"distill {temperature}")
 
@@ -448,7 +449,8 @@ def test_long_rows_when_partners_are_not_waited_for(ops, rows, cols, spins):
     calls = [lambda x, out: ops.policy_grad(x, t, adv, old, rows, ref_logp=old, kl_coef=0.1, grad=out),
              lambda x, out: ops.policy_grad(x, t, adv, old, rows, entropy_coef=0.1, grad=out),
              lambda x, out: ops.distill_grad(x, ids, tl, rows, grad=out),
-             lambda x, out: ops.distill_grad(x, ids, tl, rows, temperature=2.0, hard_coef=0.5, targets=t, grad=out)]
+             lambda x, out: ops.distill_grad(x, ids, tl, rows, temperature=2.0, hard_coef=0.5, targets=t, grad=out),
+             lambda x, out: ops.distill_grad(x, ids, tl, rows, temperature=1.5, hard_coef=0.5, targets=t, grad=out)]
     for call in calls:
         want = call(z, None)
         try:
