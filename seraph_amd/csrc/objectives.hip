@@ -1,8 +1,14 @@
 // objectives.hip - objectives over vocabulary logits beside the cross entropy: log-probabilities of given tokens, the
 // clipped policy loss, the paired preference loss and distillation from a teacher's top logits.
+//
+// Which kernel a call takes follows from its columns (and, forward only, its rows):
+//   gradient ops      up to 32768 columns: held_rows_kernel (a row in one workgroup's registers)
+//                     up to 1245184: shared_rows_kernel (a row in several workgroups' registers)
+//                     beyond: swept_rows_kernel (three sweeps over memory)
+//   forward only      up to 32768: held_rows_kernel; beyond: streamed_rows_kernel, a row in one run or in several
+//   preference        a forward pass, the pairs, and a streaming gradient pass; few rows: the last two in one
 #include <atomic>
 
-#include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
 #include "vocab_rows.hpp"
@@ -1226,7 +1232,7 @@ __global__ __launch_bounds__(kPairBlock) void small_pairs_kernel(PreferenceArgs 
     RowFactor f{0.0f, 0.0f, 0.0f, kDead};
     const int sq = find_seq(p.seq_starts, 2 * p.pairs, row);
     const uint32_t t = p.targets[row];
-    if (sq < 2 * p.pairs && row + 1 < (int64_t)p.seq_starts[sq + 1] && (int64_t)t < p.cols) {
+    if (sq < 2 * p.pairs && row >= (int64_t)p.seq_starts[sq] && row + 1 < (int64_t)p.seq_starts[sq + 1] && (int64_t)t < p.cols) {
         const Pair q = read_pair<kPairBlock>(p, sq / 2, red, false);
         f = factor_of(p, row, t, sq & 1 ? q.slope1 : q.slope0);
     }

@@ -210,7 +210,7 @@ struct Supervision {
     __device__ __forceinline__ bool in_sequence(int64_t row) const {
         if (!seq_starts) return true;
         const int sq = find_seq(seq_starts, batch, row);
-        return sq < batch && row + 1 < (int64_t)seq_starts[sq + 1];
+        return sq < batch && row >= (int64_t)seq_starts[sq] && row + 1 < (int64_t)seq_starts[sq + 1];
     }
     __device__ __forceinline__ bool live(int64_t row) const {
         if (targets && (int64_t)targets[row] >= cols) return false;

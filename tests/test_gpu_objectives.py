@@ -253,6 +253,62 @@ def test_rows_that_are_not_supervised_are_not_read(ops, cols):
     assert all((got[k] == 0).all() for k in ("grad", "loss", "logp", "kl"))
 
 
+@pytest.mark.parametrize("cols", [50, 8192, 40001])
+@pytest.mark.parametrize("rows", [11, 400])
+def test_rows_ahead_of_the_first_sequence(ops, rows, cols):
+    """Offsets that do not start at 0: what lies ahead of the first sequence is not supervised either."""
+    starts = np.array([3, 6, rows - 2], np.uint32)
+    r, z, t = make(rows, cols, cols + 11)
+    live = ref.supervised(rows, cols, t, None, starts.astype(int))
+    clean, z2 = z.copy(), z.copy()
+    z2[~live] = np.nan
+    adv, old, refl = policy_inputs(r, clean, t)
+    got = run_policy(ops, z2, t, adv, old, 7, refl=refl, kl=0.1, starts=starts, gshift=0)
+    compare(got, ref.policy(clean, t, adv, old, 7, ref=refl, clip=(0.2, 0.3), kl_coef=0.1, starts=starts.astype(int)), "policy")
+    for spoil in (0.0, float("nan")):                             # whatever the allocator hands out as scratch
+        room = torch.full((rows * 4096,), spoil, device="cuda")
+        del room
+        g, loss, scores = ops.preference_grad(dev(z2), dev(t), dev(starts), ref_logp=dev(refl))
+        compare(dict(grad=g, loss=loss, scores=scores), ref.preference(clean, t, starts.astype(int), ref=refl), "preference")
+
+
+def test_offsets_past_32_bits(ops):
+    """More logits than 2^31: the last rows of a long call give what a call of their own gives, bit for bit."""
+    rows, cols, last = 66000, 33001, 40
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    z = torch.empty(rows, cols, device="cuda").normal_(0, 2, generator=g)
+    t = torch.randint(0, cols, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    f = torch.empty(rows, device="cuda").normal_(generator=g)
+    ids = torch.randint(0, cols, (rows, 6), device="cuda", generator=g, dtype=torch.int32)
+    tl = torch.empty(rows, 6, device="cuda").normal_(generator=g)
+    t[: rows - last] = torch.where(torch.arange(rows - last, device="cuda") % 64 == 0, t[: rows - last], -1)
+    starts = torch.tensor([0, rows - last, rows], dtype=torch.int32, device="cuda")
+    part = slice(rows - last, rows)
+    zl, tl_, fl, il, ll = (a[part].clone() for a in (z, t, f, ids, tl))
+    w = torch.where(t >= 0, 1.0, 0.0)
+    want = ops.token_logprobs(zl, tl_, want_lse=True, want_entropy=True)
+    got = ops.token_logprobs(z, t, want_lse=True, want_entropy=True)
+    # (a call of 40 rows runs them whole, a long one in pieces: equal up to the order of additions)
+    for a, b in zip(got, want):
+        assert ((a[part] - b).abs() <= 1e-5).all()
+    a, b = ops.policy_grad(z, t, f, f, 10, kl_coef=0.1, ref_logp=f), ops.policy_grad(zl, tl_, fl, fl, 10, kl_coef=0.1, ref_logp=fl)
+    assert all(x is None or torch.equal(x[part], y) for x, y in zip(a, b))
+    del a
+    a, b = ops.distill_grad(z, ids, tl, 10, weights=w), ops.distill_grad(zl, il, ll, 10, weights=w[part].clone())
+    assert all(torch.equal(x[part], y) for x, y in zip(a, b))
+    del a
+    ga, la, sa = ops.preference_grad(z, t, starts, ref_logp=f, grad=z)
+    p = torch.softmax(zl.double(), 1)
+    slope = ga[rows - last, t[rows - last]].double() / (1 - p[0, tl_[0]])                # of the rejected side, from one of its entries
+    hot = torch.zeros_like(p).scatter_(1, tl_.long()[:, None], 1.0)
+    live = torch.arange(last, device="cuda") < last - 1
+    want_g = torch.where(live[:, None], slope * (hot - p), 0.0)
+    assert ((ga[part].double() - want_g).abs() <= 1e-4 * want_g.abs() + 1e-9).all() and torch.isfinite(la).all()
+
+
 @pytest.mark.parametrize("cols", [9, 1000, 8192, 33000, 151936])
 def test_masked_logits_inside_a_row(ops, cols):
     """Entries of -inf and of the type's lowest value, rows where a single entry is left, rows of nothing but lowest values,
