@@ -161,12 +161,14 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float* lds) {
     for (int w = 1; w < BLOCK / 64; w++) { a += lds[w]; b += lds[BLOCK / 64 + w]; }
 }
 
-// A row of floats that need not start on a 16-byte boundary nor hold a multiple of four: `head` single values up to the
-// first boundary, n4 vectors, `tail` single values.  Lanes 0..3 of one workgroup hold the head, lanes 4..7 the tail.
+// A row of floats that need not start on a boundary of memory's lines nor hold a multiple of four: `head` single values up to
+// the first boundary of 128 bytes, n4 vectors, `tail` single values.  Lanes 0 to 31 of one workgroup hold the head,
+// lanes 32 to 34 the tail.  (Vectors from the first 16-byte boundary on would do, but a workgroup's 4 KB would then end
+// inside a line, which two of them write a part of: 1000 x 151937 took 9 % longer than 1000 x 151936.)
 struct RowShape {
     int head, n4, tail;
     __device__ __forceinline__ RowShape(const float* row, int64_t cols) {
-        const int to_boundary = (int)((4u - ((unsigned)(reinterpret_cast<uintptr_t>(row) >> 2) & 3u)) & 3u);
+        const int to_boundary = (int)((32u - ((unsigned)(reinterpret_cast<uintptr_t>(row) >> 2) & 31u)) & 31u);
         head = to_boundary < cols ? to_boundary : (int)cols;
         n4 = (int)((cols - head) >> 2);
         tail = (int)((cols - head) & 3);
@@ -174,7 +176,7 @@ struct RowShape {
     // the column of this lane's single value, -1 where it has none
     __device__ __forceinline__ int64_t single(int lane) const {
         if (lane < head) return lane;
-        if (lane >= 4 && lane < 4 + tail) return (int64_t)head + (int64_t)n4 * 4 + (lane - 4);
+        if (lane >= 32 && lane < 32 + tail) return (int64_t)head + (int64_t)n4 * 4 + (lane - 32);
         return -1;
     }
 };

@@ -273,8 +273,10 @@ def test_rows_ahead_of_the_first_sequence(ops, rows, cols):
 
 
 def test_offsets_past_32_bits(ops):
-    """More logits than 2^31: the last rows of a long call give what a call of their own gives, bit for bit."""
-    rows, cols, last = 66000, 33001, 40
+    """More logits than 2^31: the last rows of a long call give what a call of their own gives, bit for bit where they lie
+    the same way to memory's lines (which lane takes which column follows from that, and from it the order of additions)."""
+    rows, cols, last = 66016, 33001, 32
+    assert (rows - last) * cols * 4 % 128 == 0
     free, _ = torch.cuda.mem_get_info()
     if free < 40 << 30:
         pytest.skip("needs 40 GB of device memory")
@@ -291,7 +293,7 @@ def test_offsets_past_32_bits(ops):
     w = torch.where(t >= 0, 1.0, 0.0)
     want = ops.token_logprobs(zl, tl_, want_lse=True, want_entropy=True)
     got = ops.token_logprobs(z, t, want_lse=True, want_entropy=True)
-    # (a call of 40 rows runs them whole, a long one in pieces: equal up to the order of additions)
+    # (a call of 32 rows runs them whole, a long one in pieces: equal up to the order of additions)
     for a, b in zip(got, want):
         assert ((a[part] - b).abs() <= 1e-5).all()
     a, b = ops.policy_grad(z, t, f, f, 10, kl_coef=0.1, ref_logp=f), ops.policy_grad(zl, tl_, fl, fl, 10, kl_coef=0.1, ref_logp=fl)
