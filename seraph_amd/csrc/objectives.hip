@@ -1093,26 +1093,35 @@ struct PairRowsOp {
     }
 };
 
+// A row's runs put together, in their order; four loads in flight.
 __device__ __forceinline__ RowStats joined(const PreferenceArgs& p, int64_t r) {
-    RowStats st = p.runs[r * p.splits];
-    for (int i = 1; i < p.splits; i++) {
-        const RowStats o = p.runs[r * p.splits + i];
-        const float m = fmaxf(st.m, o.m);
-        st = RowStats{m, against<kNone>(st, m, kUnitScale).s + against<kNone>(o, m, kUnitScale).s, 0.0f};
+    const RowStats* runs = p.runs + r * p.splits;
+    RowStats st = runs[0];
+    for (int i = 1; i < p.splits; i += 4) {
+        RowStats o[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = runs[i + j < p.splits ? i + j : 0];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (i + j < p.splits) {
+                const float m = fmaxf(st.m, o[j].m);
+                st = RowStats{m, against<kNone>(st, m, kUnitScale).s + against<kNone>(o[j], m, kUnitScale).s, 0.0f};
+            }
     }
     return st;
 }
-__device__ __forceinline__ RowFactor factor_of(const PreferenceArgs& p, int64_t r, uint32_t target, double f) {
-    const RowStats st = joined(p, r);
+__device__ __forceinline__ RowFactor factor_of(RowStats st, uint32_t target, double f) {
     return RowFactor{st.m, (float)(-f / (double)st.s), (float)-f, target};
 }
 
 // The two sequences of a pair, their scores and its loss; slope0 and slope1 are d(mean loss) / d(log-probability of a token) of
 // either side.  Called by a whole workgroup, half of which sums each side; sums in 64 bits and in one order whoever forms them.
-struct Pair { int64_t first, last, end; double slope0, slope1; };           // first, last, end: of this half's sequence
+// first, last, end: of this half's sequence; st: this lane's first row there
+struct Pair { int64_t first, last, end; double slope0, slope1; RowStats st; };
 template <int BLOCK>
 __device__ __forceinline__ Pair read_pair(const PreferenceArgs& p, int pair, double (*red)[BLOCK / 64], bool writes) {
     Pair q;
+    q.st = RowStats{0.0f, 1.0f, 0.0f};
     const int side = (int)threadIdx.x / (BLOCK / 2);
     const uint32_t* b = p.seq_starts + 2 * (int64_t)pair + side;
     q.first = b[0];
@@ -1122,6 +1131,7 @@ __device__ __forceinline__ Pair read_pair(const PreferenceArgs& p, int pair, dou
     for (int64_t r = q.first + (int)threadIdx.x % (BLOCK / 2); r < q.last; r += BLOCK / 2) {
         const uint32_t t = p.targets[r];
         const RowStats st = joined(p, r);                         // (not yet known to hold anything: the loads of a row do not wait for each other)
+        if (r < q.first + BLOCK / 2) q.st = st;
         const float ref = p.ref_logp ? p.ref_logp[r] : 0.0f;
         if ((int64_t)t >= p.cols || r + 1 >= q.end) continue;
         const float zt = p.splits == 1 ? st.x : p.logits[r * p.cols + t];
@@ -1184,7 +1194,7 @@ __global__ __launch_bounds__(1024) void pair_kernel(PreferenceArgs p, RowFactor*
     const double f = threadIdx.x < 512 ? q.slope0 : q.slope1;
     for (int64_t r = q.first + (int)threadIdx.x % 512; r < q.last; r += 512) {
         const uint32_t t = p.targets[r];
-        if ((int64_t)t < p.cols && r + 1 < q.end) factors[r] = factor_of(p, r, t, f);
+        if ((int64_t)t < p.cols && r + 1 < q.end) factors[r] = factor_of(r < q.first + 512 ? q.st : joined(p, r), t, f);
     }
 }
 
@@ -1234,7 +1244,7 @@ __global__ __launch_bounds__(kPairBlock) void small_pairs_kernel(PreferenceArgs 
     const uint32_t t = p.targets[row];
     if (sq < 2 * p.pairs && row >= (int64_t)p.seq_starts[sq] && row + 1 < (int64_t)p.seq_starts[sq + 1] && (int64_t)t < p.cols) {
         const Pair q = read_pair<kPairBlock>(p, sq / 2, red, false);
-        f = factor_of(p, row, t, sq & 1 ? q.slope1 : q.slope0);
+        f = factor_of(joined(p, row), t, sq & 1 ? q.slope1 : q.slope0);
     }
     pair_grad(p, grad, row, run, f);
 }
