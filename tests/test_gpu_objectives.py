@@ -272,6 +272,24 @@ def test_rows_ahead_of_the_first_sequence(ops, rows, cols):
         compare(dict(grad=g, loss=loss, scores=scores), ref.preference(clean, t, starts.astype(int), ref=refl), "preference")
 
 
+@pytest.mark.parametrize("batch,cols", [(62, 130), (63, 130), (64, 33001), (65, 130), (300, 33001), (4097, 17)])
+def test_many_sequences(ops, batch, cols):
+    """More offsets than a wave has lanes, and than it has squared; lengths from 0 to 7."""
+    batch += batch % 2
+    r = np.random.default_rng(batch)
+    starts = np.concatenate([[0], np.cumsum(r.integers(0, 8 if cols < 1000 else 4, batch))]).astype(np.uint32)
+    rows = int(starts[-1]) + 3
+    r, z, t = make(rows, cols, batch + 1)
+    adv, old, refl = policy_inputs(r, z, t)
+    s = starts.astype(int)
+    got = run_policy(ops, z, t, adv, old, 50, refl=refl, kl=0.1, starts=starts, gshift=0)
+    compare(got, ref.policy(z, t, adv, old, 50, ref=refl, clip=(0.2, 0.3), kl_coef=0.1, starts=s), "policy")
+    lp, lse, _ = ops.token_logprobs(dev(z), dev(t), seq_starts=dev(starts), want_lse=True)
+    compare(dict(logp=lp, lse=lse), ref.token_logprobs(z, t, s), "logprobs")
+    g, loss, scores = ops.preference_grad(dev(z), dev(t), dev(starts), ref_logp=dev(refl))
+    compare(dict(grad=g, loss=loss, scores=scores), ref.preference(z, t, s, ref=refl), "preference")
+
+
 def test_offsets_past_32_bits(ops):
     """More logits than 2^31: the last rows of a long call give what a call of their own gives, bit for bit where they lie
     the same way to memory's lines (which lane takes which column follows from that, and from it the order of additions)."""
