@@ -86,8 +86,10 @@ struct PolicyOp {
         const double logp = ((double)zt - (double)st.m) - log_s;
         const float w = rows.weights ? rows.weights[r] : 1.0f, adv = advantages[r];
         const float rho = exp_of((float)(logp - (double)old_logp[r]), 0.0f, kUnitScale);
-        const float free = rho * adv;
-        const float held = fminf(fmaxf(rho, 1.0f - clip_low), 1.0f + clip_high) * adv;
+        // an advantage of 0 stays 0 where the ratio is beyond the type's range (of 64 bits it would not be)
+        const bool none = adv == 0.0f && rho == INFINITY;
+        const float free = none ? 0.0f : rho * adv;
+        const float held = none ? 0.0f : fminf(fmaxf(rho, 1.0f - clip_low), 1.0f + clip_high) * adv;
         float loss = free > held ? -held : -free;                 // NaN takes the second branch of both and stays NaN
         float slope = free > held ? 0.0f : -free;                 // d loss / d logp
         if (ref_logp) {

@@ -123,6 +123,24 @@ def test_policy(ops, cols):
     assert (zero["grad"] == 0).all()
 
 
+@pytest.mark.parametrize("cols", [7, 8192, 33001])
+@pytest.mark.parametrize("high", [0.3, float("inf")])
+def test_policy_without_advantage_far_from_the_old_policy(ops, cols, high):
+    """exp(100) is beyond FP32, not beyond the 64 bits of the definition: 0 times it is 0, and the KL term remains."""
+    r, z, t = make(6, cols, cols + 11)
+    adv, old, refl = policy_inputs(r, z, t)
+    adv[[0, 1, 4]] = [0.0, -0.0, 0.0]
+    old[[0, 1]] = (target_logp(z, t)[[0, 1]] - 100.0).astype(np.float32)
+    old[5] = np.nan                                               # stays visible in its own row
+    adv[5] = 0.0
+    g, loss, logp, kl, _ = ops.policy_grad(dev(z), dev(t), dev(adv), dev(old), 6, ref_logp=dev(refl), clip=(0.2, high), kl_coef=0.1)
+    want, tol = ref.policy(z, t, adv, old, 6, ref=refl, clip=(0.2, high), kl_coef=0.1)
+    cut = lambda d, a: {k: v[:5] for k, v in d.items() if k in a}                  # noqa: E731
+    got = dict(grad=g, loss=loss, logp=logp, kl=kl)
+    compare(cut(got, got), (cut(want, got), cut(tol, got)), "policy")
+    assert torch.isnan(loss[5]) and torch.isnan(g[5]).all() and torch.isfinite(logp).all()
+
+
 @pytest.mark.parametrize("cols", COLS)
 @pytest.mark.parametrize("kind,average", [("sigmoid", False), ("hinge", True), ("squared", True)])
 def test_preference(ops, cols, kind, average):
