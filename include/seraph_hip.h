@@ -172,7 +172,8 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
  *       logsumexp of all its logits / T) is given; what the list leaves out is then left out of the loss,
  *   loss_rows[r] = w (soft_coef sum_k q_k (log q_k - log softmax(logits[r] / T)[id_k]) + hard_coef (-log softmax(logits[r])[targets[r]])),
  * grad = d(sum of loss_rows)/d logits / valid_rows (soft_coef = T^2 keeps its size as T grows).  targets (optional, needed
- * where hard_coef != 0) does not make a row unsupervised here: an id >= cols only has no hard part.  top_k is at most 1024. */
+ * where hard_coef != 0) does not make a row unsupervised here: an id >= cols only has no hard part.  With soft_coef = 0 the
+ * list is not read.  top_k is at most 1024. */
 #define SERAPH_TYPE_F32  0
 #define SERAPH_TYPE_F16  1
 #define SERAPH_TYPE_BF16 2

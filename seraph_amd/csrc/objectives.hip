@@ -1373,6 +1373,7 @@ int seraph_distill_grad(const float* logits, const uint32_t* teacher_ids, const 
     SERAPH_REQUIRE(targets || options->hard_coef == 0.0f, "distill_grad: the hard part needs targets");
     REQUIRE_WS("distill_grad", seraph_distill_grad_ws_bytes(rows, cols, top_k));
     const float scale = valid_rows > 0 ? 1.0f / (float)valid_rows : 0.0f;
+    if (options->soft_coef == 0.0f) top_k = 0;                    // the list is not read: 0 times what it holds need not be 0
     DistillOp op{{nullptr, weights, seq_starts, batch, cols}, {teacher_ids, teacher_logits, teacher_lse, options->teacher_type, (int)top_k},
                  targets, loss_rows, options->soft_coef, options->hard_coef, scale, ExpScale::of(1.0 / (double)options->temperature), 1.0 / (double)options->temperature};
     // at T = 1 the two parts share their exponentials, at T = 2 one is the other's square

@@ -207,6 +207,21 @@ def test_distill(ops, cols, top_k, dtype, temperature, hard):
         assert torch.equal(got[k], again[k]) and torch.equal(got[k], inside[k]), k
 
 
+@pytest.mark.parametrize("cols", [9, 8192, 33001, 1300003])
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_distill_without_its_soft_part(ops, cols, temperature):
+    """Nothing of the list counts then, whatever it holds."""
+    r, z, t = make(5, cols, cols + 21)
+    t[3] = cols
+    ids, teacher = distill_inputs(r, z, 5, "float32")
+    want = ref.distill(z, ids, teacher.numpy(), 5, soft=0.0, hard=0.8, targets=t, temperature=temperature)
+    teacher[1], teacher[2, 2] = float("nan"), float("inf")
+    lse = np.array([0.0, np.nan, np.inf, 1.0, -np.inf], np.float32)
+    for kw in (dict(), dict(teacher_lse=lse)):
+        got = run_distill(ops, z, ids, teacher, 5, soft_coef=0.0, hard_coef=0.8, targets=t, temperature=temperature, **kw)
+        compare(got, want, f"{cols}")
+
+
 @pytest.mark.parametrize("cols", [37, 8192, 40003])
 def test_distill_longest_list_and_the_teachers_own_norm(ops, cols):
     rows, top_k = 4, 1024
