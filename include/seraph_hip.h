@@ -125,7 +125,7 @@ void seraph_cross_entropy_exchange_spins(int spins);
  * row and its per-row results are zeros.  Rows behind the last sequence count among those.  Within a supervised row
  * a logit of -inf is an entry that cannot be chosen (probability and gradient 0).
  * Any cols and any 4-byte aligned buffers are taken.  Results do not depend on the order in which workgroups run.
- * A call without rows or columns does nothing.  ws needs 16-byte alignment; two calls that may overlap need scratch of
+ * A call without rows or columns does nothing and writes nothing; one holds at most 2^24 - 1 rows (and 2^22 - 1 pairs).  ws needs 16-byte alignment; two calls that may overlap need scratch of
  * their own.  No call allocates, waits or clears by memset, so all of them can be captured into a graph. */
 
 /* logp[r] = log softmax(logits[r])[targets[r]]; optional (NULL: not wanted) lse[r] = logsumexp of the row and

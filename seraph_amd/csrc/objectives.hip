@@ -17,6 +17,7 @@ namespace seraph {
 
 constexpr int kBlock = 256;
 constexpr int kMaxTopK = 1024;
+constexpr int64_t kMaxRows = 0xffffff;       // a launch holds less than 2^32 lanes, of which a row takes kBlock
 
 // What a row's list adds up to: the mass sum q and sum q (log q - (z - at) / T), `at` being the largest listed logit of the
 // student (the row's maximum, which the loss needs instead, may not be known yet; differences of logits keep their
@@ -953,7 +954,6 @@ static size_t streamed_ws_bytes(int64_t rows, int64_t cols) {
 
 template <class Op, int EXTRA>
 static int launch_runs(const Op& op, const float* logits, int64_t rows, int64_t cols, int splits, RowStats* runs, hipStream_t st) {
-    SERAPH_REQUIRE(rows * splits <= 0x7fffffff, "too many rows: %lld", (long long)rows);
     if (in_one_run(rows, cols))
         hipLaunchKernelGGL((streamed_rows_kernel<Op, EXTRA, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, op, logits, cols, 1, runs);
     else
@@ -1225,8 +1225,8 @@ __device__ __forceinline__ void pair_grad(const PreferenceArgs& p, float* grad, 
     if (single >= 0) out[single] = f.a * exp_of(x[single], f.m, kUnitScale) - (single == (int64_t)f.target ? f.c : 0.0f);
 }
 
-__global__ __launch_bounds__(kPairBlock) void pair_grad_kernel(PreferenceArgs p, float* grad, const RowFactor* factors, int splits_of_row) {
-    const int64_t row = (int64_t)(blockIdx.x / (unsigned)splits_of_row);
+__global__ __launch_bounds__(kPairBlock) void pair_grad_kernel(PreferenceArgs p, float* grad, const RowFactor* factors, int splits_of_row, int64_t first_row) {
+    const int64_t row = first_row + (int64_t)(blockIdx.x / (unsigned)splits_of_row);
     pair_grad(p, grad, row, (int)(blockIdx.x % (unsigned)splits_of_row), factors[row]);
 }
 
@@ -1256,7 +1256,7 @@ __global__ __launch_bounds__(kPairBlock) void small_pairs_kernel(PreferenceArgs 
 using namespace seraph;
 
 #define REQUIRE_ROWS(op)                                                                                              \
-    SERAPH_REQUIRE(rows > 0 && cols > 0 && rows <= 0x7fffffff && cols <= 0x7fffffff, op ": bad shape %lld x %lld",     \
+    SERAPH_REQUIRE(rows > 0 && cols > 0 && rows <= kMaxRows && cols <= 0x7fffffff, op ": bad shape %lld x %lld",       \
                    (long long)rows, (long long)cols)
 #define REQUIRE_WS(op, need)                                                                                          \
     do {                                                                                                              \
@@ -1323,7 +1323,7 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
     if (rows == 0 || cols == 0) return SERAPH_OK;
     REQUIRE_ROWS("preference_grad");
     SERAPH_REQUIRE(logits && targets && grad && loss_pairs && options && seq_starts, "preference_grad: NULL pointer");
-    SERAPH_REQUIRE(pairs > 0 && pairs <= 0x3fffffff, "preference_grad: bad number of pairs %d", pairs);
+    SERAPH_REQUIRE(pairs > 0 && pairs <= 0x3fffff, "preference_grad: bad number of pairs %d", pairs);
     SERAPH_REQUIRE(options->kind >= SERAPH_PREFERENCE_SIGMOID && options->kind <= SERAPH_PREFERENCE_SQUARED, "preference_grad: unknown loss %d", options->kind);
     SERAPH_REQUIRE(isfinite(options->beta) && options->beta > 0.0f, "preference_grad: beta %g must be positive", (double)options->beta);
     SERAPH_REQUIRE(options->label_smoothing >= 0.0f && options->label_smoothing <= 1.0f, "preference_grad: label smoothing %g outside [0, 1]", (double)options->label_smoothing);
@@ -1334,7 +1334,6 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
     RowFactor* factors = reinterpret_cast<RowFactor*>(ws);
     RowStats* runs = reinterpret_cast<RowStats*>(reinterpret_cast<char*>(ws) + up16((size_t)rows * sizeof(RowFactor)));
     const int64_t row_splits = ceil_div(ceil_div(cols, 4), kPairBlock);
-    SERAPH_REQUIRE(rows * row_splits <= 0x7fffffff, "preference_grad: too many logits: %lld x %lld", (long long)rows, (long long)cols);
     const bool small = splits == 1 && rows * row_splits + pairs <= 4 * (int64_t)num_compute_units();      // four workgroups of 512 lanes on a CU
     PairRowsOp op{{targets, nullptr, seq_starts, 2 * pairs, cols}, runs, small ? nullptr : factors, logp_rows, kUnitScale};
     const int rc = cols <= 32768 ? launch_rows<PairRowsOp, kNone>(op, logits, nullptr, rows, cols, 0, nullptr, st)
@@ -1349,8 +1348,12 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
     }
     hipLaunchKernelGGL(pair_kernel, dim3((unsigned)pairs), dim3(1024), 0, st, a, factors);
     SERAPH_LAUNCH_CHECK();
-    hipLaunchKernelGGL(pair_grad_kernel, dim3((unsigned)(rows * row_splits)), dim3(kPairBlock), 0, st, a, grad, factors, (int)row_splits);
-    SERAPH_LAUNCH_CHECK();
+    const int64_t at_once = 0x7fffff / row_splits;                // less than 2^32 lanes in a launch: beyond 64 GB of logits one more
+    for (int64_t first = 0; first < rows; first += at_once) {
+        const int64_t n = rows - first < at_once ? rows - first : at_once;
+        hipLaunchKernelGGL(pair_grad_kernel, dim3((unsigned)(n * row_splits)), dim3(kPairBlock), 0, st, a, grad, factors, (int)row_splits, first);
+        SERAPH_LAUNCH_CHECK();
+    }
     return SERAPH_OK;
 }
 

@@ -362,6 +362,38 @@ def test_offsets_past_32_bits(ops):
     assert ((ga[part].double() - want_g).abs() <= 1e-4 * want_g.abs() + 1e-9).all() and torch.isfinite(la).all()
 
 
+def test_pairs_whose_gradient_takes_two_launches(ops):
+    """More workgroups than one launch holds.  The slope of the hinge is known, so the definition is a softmax in 64 bits."""
+    rows, cols, beta = 8_400_001, 5, 0.25
+    g = torch.Generator(device="cuda").manual_seed(9)
+    z = torch.empty(rows, cols, device="cuda").normal_(0, 2, generator=g)
+    t = torch.randint(0, cols + 1, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    s = [0, 2_000_000, 4_100_000, 4_100_001, rows - 2]                               # a pair with a side of one token, two rows behind
+    starts = torch.tensor(s, dtype=torch.int32, device="cuda")
+    got, loss, scores = ops.preference_grad(z, t, starts, kind="hinge", beta=beta, average=True)
+    lp = torch.log_softmax(z.double(), 1)
+    live = t < cols
+    live[[b - 1 for b in s[1:]]] = False
+    live[s[-1]:] = False
+    hot = torch.zeros_like(lp).scatter_(1, t.long().clamp(max=cols - 1)[:, None], 1.0)
+    tl = torch.where(live, (lp * hot).sum(1), 0.0)
+    n = [int(live[a:b].sum()) for a, b in zip(s, s[1:])]
+    want_scores = torch.stack([tl[a:b].sum() / max(c, 1) for a, b, c in zip(s, s[1:], n)])
+    h = beta * (want_scores[0::2] - want_scores[1::2])
+    assert (h < 0.9).all()                                                           # both pairs are on the slope
+    f = torch.zeros(rows, dtype=torch.float64, device="cuda")
+    for q, (a, b, c) in enumerate(zip(s, s[1:], n)):
+        f[a:b] = (-beta if q % 2 == 0 else beta) / max(c, 1) / 2
+    f = torch.where(live, f, 0.0)[:, None]
+    p = lp.exp()
+    spread = (z.max(1).values - z.min(1).values).double()
+    u = ref.HALF_STEP * (6.0 * spread + cols / 64.0 + 40.0)                          # ref.unit
+    assert ((got.double() - f * (hot - p)).abs() <= f.abs() * 2 * u[:, None] * (p + hot) + 1e-38).all()
+    err = float(u.max())
+    assert ((scores.double() - want_scores).abs() <= err + ref.HALF_STEP * want_scores.abs()).all()
+    assert ((loss.double() - (1.0 - h)).abs() <= 2 * beta * err + ref.HALF_STEP * (1.0 - h).abs()).all()
+
+
 @pytest.mark.parametrize("cols", [9, 1000, 8192, 33000, 151936])
 def test_masked_logits_inside_a_row(ops, cols):
     """Entries of -inf and of the type's lowest value, rows where a single entry is left, rows of nothing but lowest values,

@@ -163,3 +163,14 @@ def test_wrappers_refuse_what_is_not_on_the_device():
                  lambda: ops.preference_grad(z, ids, ids), lambda: ops.distill_grad(z, ids, z, 4)):
         with pytest.raises(SeraphError, match="CUDA"):
             call()
+
+
+def test_more_rows_than_a_launch_holds(k):
+    from seraph_amd._lib import DistillOptions, PolicyOptions, PreferenceOptions
+    rows = 1 << 24
+    refused(k, k.seraph_token_logprobs(P, P, P, None, None, None, 1, rows, 8, None, 0, None), -1, "shape")
+    refused(k, k.seraph_policy_grad(P, P, P, P, None, None, P, P, None, None, None, PolicyOptions(0.2, 0.2, 0.0, 0.0), None, 1, rows, 8, 4, None, 0, None), -1, "shape")
+    refused(k, k.seraph_distill_grad(P, P, P, None, None, None, P, P, DistillOptions(1.0, 1.0, 0.0, 0), None, 1, rows, 8, 2, 4, None, 0, None), -1, "shape")
+    o = PreferenceOptions(0, 0.1, 0.0, 0.0, 0)
+    refused(k, k.seraph_preference_grad(P, P, None, P, P, None, None, o, P, 1, rows, 8, P, 1 << 60, None), -1, "shape")
+    refused(k, k.seraph_preference_grad(P, P, None, P, P, None, None, o, P, 1 << 22, 4, 8, P, 1 << 60, None), -1, "pairs")
