@@ -1258,6 +1258,10 @@ using namespace seraph;
 #define REQUIRE_ROWS(op)                                                                                              \
     SERAPH_REQUIRE(rows > 0 && cols > 0 && rows <= kMaxRows && cols <= 0x7fffffff, op ": bad shape %lld x %lld",       \
                    (long long)rows, (long long)cols)
+// A gradient that covers other logits than its own would overwrite what another workgroup still reads.
+#define REQUIRE_GRAD(op)                                                                                              \
+    SERAPH_REQUIRE(grad == logits || (uintptr_t)grad >= (uintptr_t)(logits + rows * cols) || (uintptr_t)logits >= (uintptr_t)(grad + rows * cols), \
+                   op ": grad has to be the logits themselves or not overlap them")
 #define REQUIRE_WS(op, need)                                                                                          \
     do {                                                                                                              \
         if ((need) && (!ws || ws_bytes < (need) || !aligned16(ws))) {                                                 \
@@ -1302,6 +1306,7 @@ int seraph_policy_grad(const float* logits, const uint32_t* actions, const float
                    (double)options->clip_low, (double)options->clip_high);
     SERAPH_REQUIRE(isfinite(options->kl_coef) && isfinite(options->entropy_coef), "policy_grad: coefficients must be finite");
     SERAPH_REQUIRE(ref_logp || (options->kl_coef == 0.0f && !kl_rows), "policy_grad: the KL term needs ref_logp");
+    REQUIRE_GRAD("policy_grad");
     REQUIRE_WS("policy_grad", seraph_policy_grad_ws_bytes(rows, cols));
     const float scale = valid_rows > 0 ? 1.0f / (float)valid_rows : 0.0f;
     PolicyOp op{{actions, weights, seq_starts, batch, cols}, advantages, old_logp, ref_logp, loss_rows, logp_rows, kl_rows, entropy_rows,
@@ -1328,6 +1333,7 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
     SERAPH_REQUIRE(isfinite(options->beta) && options->beta > 0.0f, "preference_grad: beta %g must be positive", (double)options->beta);
     SERAPH_REQUIRE(options->label_smoothing >= 0.0f && options->label_smoothing <= 1.0f, "preference_grad: label smoothing %g outside [0, 1]", (double)options->label_smoothing);
     SERAPH_REQUIRE(isfinite(options->margin), "preference_grad: margin must be finite");
+    REQUIRE_GRAD("preference_grad");
     REQUIRE_WS("preference_grad", seraph_preference_grad_ws_bytes(rows, cols));
     hipStream_t st = as_stream(s);
     const int splits = pair_runs(rows, cols);
@@ -1374,6 +1380,7 @@ int seraph_distill_grad(const float* logits, const uint32_t* teacher_ids, const 
     SERAPH_REQUIRE(isfinite(options->soft_coef) && isfinite(options->hard_coef), "distill_grad: coefficients must be finite");
     SERAPH_REQUIRE(options->teacher_type >= SERAPH_TYPE_F32 && options->teacher_type <= SERAPH_TYPE_BF16, "distill_grad: unknown teacher type %d", options->teacher_type);
     SERAPH_REQUIRE(targets || options->hard_coef == 0.0f, "distill_grad: the hard part needs targets");
+    REQUIRE_GRAD("distill_grad");
     REQUIRE_WS("distill_grad", seraph_distill_grad_ws_bytes(rows, cols, top_k));
     const float scale = valid_rows > 0 ? 1.0f / (float)valid_rows : 0.0f;
     if (options->soft_coef == 0.0f) top_k = 0;                    // the list is not read: 0 times what it holds need not be 0

@@ -174,3 +174,12 @@ def test_more_rows_than_a_launch_holds(k):
     o = PreferenceOptions(0, 0.1, 0.0, 0.0, 0)
     refused(k, k.seraph_preference_grad(P, P, None, P, P, None, None, o, P, 1, rows, 8, P, 1 << 60, None), -1, "shape")
     refused(k, k.seraph_preference_grad(P, P, None, P, P, None, None, o, P, 1 << 22, 4, 8, P, 1 << 60, None), -1, "pairs")
+
+
+@pytest.mark.parametrize("off", [4, -4, 4 * 31, -4 * 31])
+def test_a_gradient_over_other_logits_than_its_own(k, off):
+    from seraph_amd._lib import DistillOptions, PolicyOptions, PreferenceOptions
+    g = P + off                                                                          # 4 x 8 logits: 128 bytes
+    refused(k, k.seraph_policy_grad(P, P, P, P, None, None, g, P, None, None, None, PolicyOptions(0.2, 0.2, 0.0, 0.0), None, 1, 4, 8, 4, None, 0, None), -1, "overlap")
+    refused(k, k.seraph_distill_grad(P, P, P, None, None, None, g, P, DistillOptions(1.0, 1.0, 0.0, 0), None, 1, 4, 8, 2, 4, None, 0, None), -1, "overlap")
+    refused(k, k.seraph_preference_grad(P, P, None, g, P, None, None, PreferenceOptions(0, 0.1, 0.0, 0.0, 0), P, 1, 4, 8, P, 1 << 60, None), -1, "overlap")
