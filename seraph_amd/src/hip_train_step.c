@@ -849,7 +849,7 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
     const float scale = 1.0f / sqrtf((float)D);
     const float eps = c->rms_eps, theta = c->rope_theta > 0 ? c->rope_theta : 10000.0f;
     int num_valid = total_tokens - batch;                               /* src/train_cuda.c:1989-1991 */
-    if (num_valid <= 0) return 0.0f;
+    if (num_valid <= 0 && !(obj && obj->kind == OBJ_PREFERENCE)) return 0.0f;      /* (a pair has its loss without a prediction too) */
     if (obj && obj->kind != OBJ_LOGPROBS) {                             /* the predictions that count: not the prompts', not a sequence's last */
         num_valid = 0;
         for (int b = 0; b < batch; b++) {
@@ -897,7 +897,7 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
                                                   {a->xn_attn, W + t->L.v, a->v, T, kv}};
             GEMM_GROUP(qkv, 3, h, 0, 1, 0);
         }
-        if (adapters) {                                                        /* the q, k and v adapters in one launch per product */
+        if (adapters) {                                                    /* the q, k and v adapters in one launch per product */
             float* outs[3] = {a->q, a->k, a->v};
             const int64_t od[3] = {qd, kv, kv};
             lora_fwd_item_t it[3];
@@ -971,7 +971,7 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
     }
     float* red_in = t->loss_rows;
     float* red_out = t->red_a;
-    for (size_t n = loss_count; n > 1; n = (n + 511) / 512) {                              /* src/train.c:4902-4913 */
+    for (size_t n = loss_count; n > 1; n = (n + 511) / 512) {                             /* src/train.c:4902-4913 */
         CK(seraph_reduce_sum(red_in, red_out, n, s));
         red_in = red_out;
         red_out = (red_out == t->red_a) ? t->red_b : t->red_a;
@@ -1241,10 +1241,11 @@ int hip_train_step_policy(hip_trainer_t* t, const int* tokens_packed, int total_
 int hip_train_step_preference(hip_trainer_t* t, const int* tokens_packed, int total_tokens, const int* seq_starts, int pairs,
                               const uint8_t* supervised, const float* ref_logp, const seraph_preference_options_t* options,
                               int run_optimizer, float* loss, float* scores) {
-    if (!t || !options || !seq_starts || pairs < 1 || pairs > 0x3fffffff) {
+    if (!t || !options || !seq_starts || pairs < 1 || pairs > 0x3fffff) {
         fprintf(stderr, "ERROR: hip_train_step_preference: options and the offsets of 2 * pairs sequences are needed\n");
         return -1;
     }
+    for (int64_t i = 0; scores && i < 2 * (int64_t)pairs; i++) scores[i] = 0.0f;
     objective_t o = {0};
     o.kind = OBJ_PREFERENCE;
     o.supervised = supervised; o.ref_logp = ref_logp; o.host_scores = scores;

@@ -232,3 +232,14 @@ def test_batches_without_a_prediction_and_refusals(tr, orc, capfd):
     assert np.isnan(t.step_policy(tok, STARTS, np.full(T, np.nan, np.float32), f)) and t.nan_detected
     assert (t.download(tr.PARAMS) == p).all()
     t.close()
+
+
+def test_pairs_of_single_tokens(tr, orc):
+    """Nothing is predicted anywhere: the loss of equal scores, no gradient, and the step counts as one."""
+    _, p, tok, t = setup(tr, orc, MODEL, 47)
+    ones = np.arange(5, dtype=np.int32)
+    loss, scores = t.step_preference(tok[:4], ones, kind="hinge", beta=0.5, margin=0.25, run_optimizer=False)
+    assert loss == 1.25 and (scores == 0).all() and (t.download(tr.GRADS) == 0).all()
+    loss, scores = t.step_preference(tok[:4], ones, beta=0.5)
+    assert abs(loss - np.log(2)) < 1e-6 and (scores == 0).all() and t.optimizer_step == 1
+    t.close()
