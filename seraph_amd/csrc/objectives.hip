@@ -95,11 +95,11 @@ struct PolicyOp {
         float slope = free > held ? 0.0f : -free;                 // d loss / d logp
         if (ref_logp) {
             const double d = (double)ref_logp[r] - logp;
-            const float kl = exp_excess(d, exp_of((float)d, 0.0f, kUnitScale));
+            const float e = exp_of((float)d, 0.0f, kUnitScale), kl = exp_excess(d, e);
             if (kl_rows && writes) kl_rows[r] = kl;
             if (kl_coef != 0.0f) {
                 loss = fmaf(kl_coef, kl, loss);
-                slope = fmaf(-kl_coef, kl + (float)d, slope);     // e^d - 1
+                slope = fmaf(-kl_coef, exp_less_one(d, e, kl), slope);
             }
         }
         const float sc = w * scale, inv_total = 1.0f / st.s;

@@ -75,6 +75,9 @@ __device__ __forceinline__ float exp_excess(double d, float e) {
     p = fmaf(p, x, 0.5f);
     return x * x * p;
 }
+// e^d - 1 from the same.  Near zero, where e - 1 would cancel, it is the excess plus d; beyond, the excess has lost the 1 beside a
+// large |d| (all of it below -2^24) and is infinite at d = -inf, where e - 1 is the -1 that it should be.
+__device__ __forceinline__ float exp_less_one(double d, float e, float excess) { return fabs(d) < 1.0 ? excess + (float)d : e - 1.0f; }
 
 template <int EXTRA>
 __device__ __forceinline__ float extra_of(float z, float m, float e) {
