@@ -1165,7 +1165,10 @@ __device__ __forceinline__ Pair read_pair(const PreferenceArgs& p, int pair, dou
     double slope;                                                 // d loss / d gap
     if (p.kind == SERAPH_PREFERENCE_SIGMOID) {
         const double eps = (double)p.smoothing, soft = log1p(exp(-fabs(h)));
-        loss = h != h ? h : (1.0 - eps) * (soft + fmax(-h, 0.0)) + eps * (soft + fmax(h, 0.0));
+        loss = h != h ? h : 0.0;
+        // (a term whose factor is 0 is left out: a gap is infinite where an answer holds a token that cannot be chosen)
+        if (eps != 1.0) loss += (1.0 - eps) * (soft + fmax(-h, 0.0));
+        if (eps != 0.0) loss += eps * (soft + fmax(h, 0.0));
         slope = beta * (eps - 1.0 / (1.0 + exp(h)));
     } else if (p.kind == SERAPH_PREFERENCE_HINGE) {
         loss = h >= 1.0 ? 0.0 : 1.0 - h;

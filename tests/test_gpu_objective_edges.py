@@ -27,3 +27,35 @@ def test_kl_term_of_tokens_that_the_reference_masks(ops, cols, ent):
         want = ref.policy(z, t, adv, old, rows, ref=refl, clip=(0.2, 0.3), kl_coef=0.25, entropy_coef=ent)
     assert np.isfinite(want[0]["grad"]).all()
     compare(got, want, f"{cols}")
+
+
+# rows x columns of every form that the preference loss has: one pass per pair and gradient, rows in one workgroup or in one run;
+# pairs of their own kernel, rows in one workgroup or in several runs
+PAIR_FORMS = [(30, 50), (30, 8192), (30, 40001), (1300, 50), (300, 40001)]
+
+
+def pair_inputs(rows, cols, seed, pairs=4):
+    r, z, t = make(rows, cols, seed)
+    cuts = np.linspace(0, rows, 2 * pairs + 1).astype(int)
+    cuts[1:-1] += r.integers(0, 2, 2 * pairs - 1)                 # ragged, two tokens at least
+    refl = (target_logp(z, t) + 0.3 * r.standard_normal(rows)).astype(np.float32)
+    return z, t, cuts, refl
+
+
+@pytest.mark.parametrize("rows,cols", PAIR_FORMS)
+@pytest.mark.parametrize("eps", [0.0, 0.1, 1.0])
+def test_sigmoid_loss_of_an_infinite_gap(ops, rows, cols, eps):
+    """An answer with a token that cannot be chosen has the score -inf.  -log sigmoid(inf) is 0, and a term whose factor is 0 is
+    not there: the loss is 0 where the preferred side wins for certain, infinite where it loses."""
+    z, t, starts, refl = pair_inputs(rows, cols, cols + 41)
+    for side in (3, 4):                                           # pair 1: its rejected answer; pair 2: its chosen one
+        row = starts[side]
+        z[row, t[row]] = -np.inf
+    got = ops.preference_grad(dev(z), dev(t), dev(starts.astype(np.uint32)), ref_logp=dev(refl), beta=0.3, label_smoothing=eps)
+    with np.errstate(invalid="ignore", over="ignore"):
+        want, tol = ref.preference(z, t, starts, ref=refl, beta=0.3, eps=eps)
+    want["loss"][1] = 0.0 if eps == 0 else np.inf
+    want["loss"][2] = 0.0 if eps == 1 else np.inf
+    assert want["scores"][3] == -np.inf and want["scores"][4] == -np.inf and np.isfinite(want["grad"]).all()
+    tol["loss"][1:3] = 0.0
+    compare(dict(grad=got[0], loss=got[1], scores=got[2]), (want, tol), f"{rows} x {cols}")
