@@ -1172,7 +1172,7 @@ __device__ __forceinline__ Pair read_pair(const PreferenceArgs& p, int pair, dou
         slope = beta * (eps - 1.0 / (1.0 + exp(h)));
     } else if (p.kind == SERAPH_PREFERENCE_HINGE) {
         loss = h >= 1.0 ? 0.0 : 1.0 - h;
-        slope = h >= 1.0 ? 0.0 : -beta;
+        slope = h >= 1.0 ? 0.0 : h < 1.0 ? -beta : h;             // (NaN stays NaN)
     } else {
         const double d = gap - 0.5 / beta;
         loss = d * d;

@@ -59,3 +59,26 @@ def test_sigmoid_loss_of_an_infinite_gap(ops, rows, cols, eps):
     assert want["scores"][3] == -np.inf and want["scores"][4] == -np.inf and np.isfinite(want["grad"]).all()
     tol["loss"][1:3] = 0.0
     compare(dict(grad=got[0], loss=got[1], scores=got[2]), (want, tol), f"{rows} x {cols}")
+
+
+@pytest.mark.parametrize("rows,cols", PAIR_FORMS)
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "squared"])
+def test_a_pair_without_a_score_shows_it(ops, rows, cols, kind):
+    """NaN in one entry of ref_logp: the loss of its pair and the gradients of all of the pair's supervised rows are NaN, which a
+    step's checks see; the other pairs keep their bits."""
+    z, t, starts, refl = pair_inputs(rows, cols, cols + 43)
+    t[starts[2] + 1] = cols                                       # one row of the pair that is not supervised, beside the last ones
+    live = ref.supervised(rows, cols, t, None, starts)
+    spoilt = refl.copy()
+    spoilt[starts[3]] = np.nan                                    # (a rejected answer; its pair is rows starts[2] to starts[4])
+
+    def run(refl):
+        got = ops.preference_grad(dev(z), dev(t), dev(starts.astype(np.uint32)), ref_logp=dev(refl), kind=kind, beta=0.3)
+        return [a.cpu().numpy() for a in got]
+    (g0, l0, s0), (g, l, s) = run(refl), run(spoilt)
+    pair = np.zeros(rows, bool)
+    pair[starts[2]:starts[4]] = True
+    assert live[starts[3]] and np.isfinite(g0).all() and np.isfinite(l0).all() and np.isfinite(s0).all()
+    assert np.isnan(g[pair & live]).all() and (g[pair & ~live] == 0).all() and np.array_equal(g[~pair], g0[~pair])
+    assert np.array_equal(np.isnan(l), np.arange(4) == 1) and np.array_equal(l[[0, 2, 3]], l0[[0, 2, 3]])
+    assert np.array_equal(np.isnan(s), np.arange(8) == 3) and np.array_equal(np.delete(s, 3), np.delete(s0, 3))
