@@ -118,8 +118,8 @@ void seraph_cross_entropy_exchange_spins(int spins);
  * What a training step puts in the place of seraph_cross_entropy_grad when it does not learn the next token of a text:
  * policy optimisation on sampled answers, preference pairs, distillation.  The reference trains with the cross entropy
  * alone, so these have no counterpart there; they keep its conventions: FP32 logits [rows, cols], the loss per row
- * undivided and the gradient divided by valid_rows (0 -> all gradients 0), grad may be the logits (but not overlap them
- * otherwise).
+ * undivided and the gradient divided by valid_rows (0 -> all gradients 0).  grad may be the logits; otherwise no output and no
+ * scratch may share memory with another buffer of the call (refused; old_logp cannot be updated in place by logp_rows).
  *
  * A row is supervised when its target is below cols, its weight (where the op has weights) is not 0 and, with
  * seq_starts, it lies in a sequence and is not that sequence's last token.  Any other row is not read: its gradient

@@ -1273,6 +1273,33 @@ using namespace seraph;
         }                                                                                                             \
     } while (0)
 
+namespace seraph {
+// The buffers of a call (NULL and empty ones count for nothing).  What it writes shares memory with none of the others: every
+// workgroup that works on a row reads the row's inputs, at times that nothing orders against another one's writes.
+struct Extent { const void* at; size_t bytes; bool written; };
+template <int N>
+static bool apart(const Extent (&e)[N]) {
+    for (int i = 0; i < N; i++) {
+        if (!e[i].written || !e[i].at || !e[i].bytes) continue;
+        const uintptr_t a = (uintptr_t)e[i].at;
+        for (int j = 0; j < N; j++) {
+            const uintptr_t b = (uintptr_t)e[j].at;
+            if (j != i && b && a < b + e[j].bytes && b < a + e[i].bytes) return false;
+        }
+    }
+    return true;
+}
+static size_t words(int64_t n) { return (size_t)n * 4; }
+static size_t offsets_bytes(const uint32_t* seq_starts, int64_t batch) { return seq_starts ? words(batch + 1) : 0; }
+// (a gradient in the logits' place is one buffer)
+static size_t logits_bytes(const float* logits, const float* grad, int64_t rows, int64_t cols) { return logits == grad ? 0 : words(rows * cols); }
+}  // namespace seraph
+#define REQUIRE_APART(op, ...)                                                                                        \
+    do {                                                                                                              \
+        const Extent extents[] = {__VA_ARGS__};                                                                       \
+        SERAPH_REQUIRE(apart(extents), op ": an output overlaps another buffer of the call");                         \
+    } while (0)
+
 extern "C" {
 
 void seraph_objectives_exchange_spins(int spins) {
@@ -1289,6 +1316,9 @@ int seraph_token_logprobs(const float* logits, const uint32_t* targets, float* l
     SERAPH_REQUIRE(logits && targets && logp, "token_logprobs: NULL pointer");
     SERAPH_REQUIRE(!seq_starts || batch >= 1, "token_logprobs: packed call needs batch >= 1");
     REQUIRE_WS("token_logprobs", seraph_token_logprobs_ws_bytes(rows, cols));
+    REQUIRE_APART("token_logprobs", {logits, words(rows * cols), false}, {targets, words(rows), false}, {seq_starts, offsets_bytes(seq_starts, batch), false},
+                  {logp, words(rows), true}, {lse, words(rows), true}, {entropy, words(rows), true},
+                  {ws, seraph_token_logprobs_ws_bytes(rows, cols), true});
     LogprobsOp op{{targets, nullptr, seq_starts, batch, cols}, logp, lse, entropy, kUnitScale};
     if (entropy) return launch_rows<LogprobsOp, kEntropy>(op, logits, nullptr, rows, cols, 0, ws, as_stream(s));
     return launch_rows<LogprobsOp, kNone>(op, logits, nullptr, rows, cols, 0, ws, as_stream(s));
@@ -1311,6 +1341,11 @@ int seraph_policy_grad(const float* logits, const uint32_t* actions, const float
     SERAPH_REQUIRE(ref_logp || (options->kl_coef == 0.0f && !kl_rows), "policy_grad: the KL term needs ref_logp");
     REQUIRE_GRAD("policy_grad");
     REQUIRE_WS("policy_grad", seraph_policy_grad_ws_bytes(rows, cols));
+    REQUIRE_APART("policy_grad", {logits, logits_bytes(logits, grad, rows, cols), false}, {actions, words(rows), false}, {advantages, words(rows), false},
+                  {old_logp, words(rows), false}, {ref_logp, words(rows), false}, {weights, words(rows), false},
+                  {seq_starts, offsets_bytes(seq_starts, batch), false}, {grad, words(rows * cols), true}, {loss_rows, words(rows), true},
+                  {logp_rows, words(rows), true}, {kl_rows, words(rows), true}, {entropy_rows, words(rows), true},
+                  {ws, seraph_policy_grad_ws_bytes(rows, cols), true});
     const float scale = valid_rows > 0 ? 1.0f / (float)valid_rows : 0.0f;
     PolicyOp op{{actions, weights, seq_starts, batch, cols}, advantages, old_logp, ref_logp, loss_rows, logp_rows, kl_rows, entropy_rows,
                 options->clip_low, options->clip_high, options->kl_coef, options->entropy_coef, scale, kUnitScale};
@@ -1338,6 +1373,9 @@ int seraph_preference_grad(const float* logits, const uint32_t* targets, const f
     SERAPH_REQUIRE(isfinite(options->margin), "preference_grad: margin must be finite");
     REQUIRE_GRAD("preference_grad");
     REQUIRE_WS("preference_grad", seraph_preference_grad_ws_bytes(rows, cols));
+    REQUIRE_APART("preference_grad", {logits, logits_bytes(logits, grad, rows, cols), false}, {targets, words(rows), false}, {ref_logp, words(rows), false},
+                  {seq_starts, offsets_bytes(seq_starts, 2 * (int64_t)pairs), false}, {grad, words(rows * cols), true}, {loss_pairs, words(pairs), true},
+                  {scores, words(2 * (int64_t)pairs), true}, {logp_rows, words(rows), true}, {ws, seraph_preference_grad_ws_bytes(rows, cols), true});
     hipStream_t st = as_stream(s);
     const int splits = pair_runs(rows, cols);
     RowFactor* factors = reinterpret_cast<RowFactor*>(ws);
@@ -1385,6 +1423,10 @@ int seraph_distill_grad(const float* logits, const uint32_t* teacher_ids, const 
     SERAPH_REQUIRE(targets || options->hard_coef == 0.0f, "distill_grad: the hard part needs targets");
     REQUIRE_GRAD("distill_grad");
     REQUIRE_WS("distill_grad", seraph_distill_grad_ws_bytes(rows, cols, top_k));
+    REQUIRE_APART("distill_grad", {logits, logits_bytes(logits, grad, rows, cols), false}, {teacher_ids, words(rows * top_k), false},
+                  {teacher_logits, words(rows * top_k) / (options->teacher_type == SERAPH_TYPE_F32 ? 1 : 2), false}, {teacher_lse, words(rows), false},
+                  {targets, words(rows), false}, {weights, words(rows), false}, {seq_starts, offsets_bytes(seq_starts, batch), false},
+                  {grad, words(rows * cols), true}, {loss_rows, words(rows), true}, {ws, seraph_distill_grad_ws_bytes(rows, cols, top_k), true});
     const float scale = valid_rows > 0 ? 1.0f / (float)valid_rows : 0.0f;
     if (options->soft_coef == 0.0f) top_k = 0;                    // the list is not read: 0 times what it holds need not be 0
     DistillOp op{{nullptr, weights, seq_starts, batch, cols}, {teacher_ids, teacher_logits, teacher_lse, options->teacher_type, (int)top_k},

@@ -82,3 +82,24 @@ def test_a_pair_without_a_score_shows_it(ops, rows, cols, kind):
     assert np.isnan(g[pair & live]).all() and (g[pair & ~live] == 0).all() and np.array_equal(g[~pair], g0[~pair])
     assert np.array_equal(np.isnan(l), np.arange(4) == 1) and np.array_equal(l[[0, 2, 3]], l0[[0, 2, 3]])
     assert np.array_equal(np.isnan(s), np.arange(8) == 3) and np.array_equal(np.delete(s, 3), np.delete(s0, 3))
+
+
+@pytest.mark.parametrize("rows,cols", [(7, 13), (5, 33001)])
+def test_buffers_that_touch(ops, rows, cols):
+    """Slices of one allocation, each starting where the one before ends, share nothing."""
+    r, z, t = make(rows, cols, cols + 47)
+    adv, old, refl = policy_inputs(r, z, t)
+    w = (0.5 + r.random(rows)).astype(np.float32)
+    parts = [adv, np.full(z.shape, np.nan, np.float32), old, z, refl, w]
+    room = torch.empty(sum(p.size for p in parts), device="cuda")
+    views, at = [], 0
+    for p in parts:
+        views.append(room[at:at + p.size].view(p.shape))
+        views[-1].copy_(torch.from_numpy(p))
+        at += p.size
+    a, grad, o, Z, R, W = views
+    got = ops.policy_grad(Z, dev(t), a, o, rows, ref_logp=R, weights=W, clip=(0.2, 0.3), kl_coef=0.05, grad=grad)
+    want = ref.policy(z, t, adv, old, rows, ref=refl, weights=w, clip=(0.2, 0.3), kl_coef=0.05)
+    compare(dict(zip(("grad", "loss", "logp", "kl"), got)), want, f"{cols}")
+    for view, p in zip((a, o, Z, R, W), (adv, old, z, refl, w)):
+        assert np.array_equal(view.cpu().numpy(), p)
