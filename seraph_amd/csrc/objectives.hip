@@ -94,12 +94,11 @@ struct PolicyOp {
         float loss = free > held ? -held : -free;                 // NaN takes the second branch of both and stays NaN
         float slope = free > held ? 0.0f : -free;                 // d loss / d logp
         if (ref_logp) {
-            const double d = (double)ref_logp[r] - logp;
-            const float e = exp_of((float)d, 0.0f, kUnitScale), kl = exp_excess(d, e);
-            if (kl_rows && writes) kl_rows[r] = kl;
+            const ExpLess kl = exp_less((double)ref_logp[r] - logp);
+            if (kl_rows && writes) kl_rows[r] = kl.excess;
             if (kl_coef != 0.0f) {
-                loss = fmaf(kl_coef, kl, loss);
-                slope = fmaf(-kl_coef, exp_less_one(d, e, kl), slope);
+                loss = fmaf(kl_coef, kl.excess, loss);
+                slope = fmaf(-kl_coef, kl.rise, slope);
             }
         }
         const float sc = w * scale, inv_total = 1.0f / st.s;

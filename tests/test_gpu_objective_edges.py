@@ -103,3 +103,23 @@ def test_buffers_that_touch(ops, rows, cols):
     compare(dict(zip(("grad", "loss", "logp", "kl"), got)), want, f"{cols}")
     for view, p in zip((a, o, Z, R, W), (adv, old, z, refl, w)):
         assert np.array_equal(view.cpu().numpy(), p)
+
+
+def test_kl_estimate_far_from_the_reference(ops):
+    """k(d) = e^d - 1 - d over the range of FP32.  In rows of one column logp is 0 up to the 1e-7 of a row's logarithm, so d is ref_logp up
+    to that, which changes k by at most 1e-7 |e^d - 1|.  Beyond |d| = 1 an exponential good to a step of its last place (2^-23, and half
+    of that for rounding its argument's fraction) and the difference's rounding remain; below, the terms of the series: six
+    half steps for their products and sums, one for what is cut off, one for the last product."""
+    d = np.concatenate([np.linspace(-100.0, 88.0, 1501), np.linspace(-1.5, 1.5, 401), np.geomspace(1e-3, 1.0, 60), -np.geomspace(1e-3, 1.0, 60)]).astype(np.float32)
+    rows = len(d)
+    z, t, zero = np.linspace(-3, 3, rows).astype(np.float32)[:, None], np.zeros(rows, np.uint32), np.zeros(rows, np.float32)
+    _, loss, logp, kl, _ = ops.policy_grad(dev(z), dev(t), dev(zero), dev(zero), rows, ref_logp=dev(d), kl_coef=0.5)
+    d = d.astype(np.float64)
+    rise = np.expm1(d)
+    # e^d - 1 - d without its cancellation
+    want = np.where(np.abs(d) < 1e-2, d * d * (0.5 + d * (1 / 6 + d * (1 / 24 + d * (1 / 120 + d / 720)))), rise - d)
+    far = np.abs(d) >= 1
+    tol = 1e-7 * np.abs(rise) + 1e-14 * np.exp(d) + ref.HALF_STEP * np.where(far, 3 * np.exp(d) + 2 * want, 8 * want)
+    assert np.abs(logp.cpu().numpy()).max() <= 1e-7
+    check("k", kl, want, tol)
+    check("loss", loss, 0.5 * want, 0.5 * tol + ref.HALF_STEP * 0.5 * want)
