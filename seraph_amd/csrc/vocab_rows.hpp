@@ -60,23 +60,20 @@ __device__ __forceinline__ double log_of(float s) {
     return (double)__builtin_amdgcn_frexp_expf(s) * 0.693147180559945309 + (double)(__builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(s)) * 0.6931471805599453f);
 }
 
-// e^d of a 64-bit d to one or two units of its last place: 2^n times the exponential of a fraction that FP32 holds to 2^-25.
-// (exp_of rounds its argument to FP32, which costs |d| / 2 units.)
+// e^d of a 64-bit d to one or two units of its last place: d in two floats, and 2^n times the exponential of a fraction that FP32
+// holds to 2^-25.  (exp_of rounds its argument to FP32, which costs |d| / 2 units.)
 __device__ __forceinline__ float exp_of_wide(double d) {
-    const double t = d * 1.4426950408889634074, n = rint(t);
-    if (!(fabs(t) < 200.0)) return t < 0.0 ? 0.0f : t > 0.0 ? INFINITY : (float)t;
-    return ldexpf(__builtin_amdgcn_exp2f((float)(t - n)), (int)n);
+    const float hi = (float)d, t = hi * kUnitScale.hi, n = rintf(t), lo = (float)(d - (double)hi);
+    const float e = ldexpf(__builtin_amdgcn_exp2f(fmaf(hi, kUnitScale.hi, -n) + fmaf(hi, kUnitScale.lo, lo * kUnitScale.hi)), (int)n);
+    return fabsf(t) < 200.0f ? e : t < 0.0f ? 0.0f : t > 0.0f ? INFINITY : t;
 }
 
 // e^d - 1 (rise) and e^d - 1 - d (excess), each to a few units of its last place.  Near zero, where the differences would cancel, the
 // excess by its series and the rise as excess + d; from |d| = 1 on both from e^d itself: there the excess would lose the 1
-// beside a large |d|, and it is infinite at d = -inf, where the rise is -1.
+// beside a large |d|, and it is infinite at d = -inf, where the rise is -1.  Without branches: one lane computes it
+// while its workgroup waits, and a branch around e^d took 0.07 us of the 21 that the policy loss takes at 2048 x 8192.
 struct ExpLess { float rise, excess; };
 __device__ __forceinline__ ExpLess exp_less(double d) {
-    if (!(fabs(d) < 1.0)) {
-        const double rise = (double)exp_of_wide(d) - 1.0;
-        return ExpLess{(float)rise, (float)(rise - d)};
-    }
     const float x = (float)d;
     float p = 1.0f / 3628800.0f;                                  // x^2 (1/2! + x/3! + ... + x^8/10!)
     p = fmaf(p, x, 1.0f / 362880.0f);
@@ -87,8 +84,10 @@ __device__ __forceinline__ ExpLess exp_less(double d) {
     p = fmaf(p, x, 1.0f / 24.0f);
     p = fmaf(p, x, 1.0f / 6.0f);
     p = fmaf(p, x, 0.5f);
-    const float excess = x * x * p;
-    return ExpLess{excess + x, excess};
+    const bool near = fabs(d) < 1.0;
+    const float series = x * x * p;
+    const double rise = (double)exp_of_wide(d) - 1.0;
+    return ExpLess{near ? series + x : (float)rise, near ? series : (float)(rise - d)};
 }
 
 template <int EXTRA>
