@@ -182,9 +182,10 @@ def policy_grad(logits, actions, advantages, old_logp, valid_rows, ref_logp=None
 
 
 def preference_grad(logits, targets, seq_starts, ref_logp=None, kind="sigmoid", beta=0.1, label_smoothing=0.0, margin=0.0,
-                    average=False, grad=None):
+                    average=False, grad=None, logp=None):
     """Preference loss over the pairs (2i chosen, 2i + 1 rejected) of the packed sequences: (gradient of the mean loss with
-    respect to the logits, loss of each pair, score of each sequence).  grad may be the logits themselves."""
+    respect to the logits, loss of each pair, score of each sequence).  grad may be the logits themselves; logp, a tensor
+    of one float32 for each row, takes the log-probabilities that the scores add up (0 where a row is not supervised)."""
     op = "preference_grad"
     rows, cols, device = _logits(op, logits)
     t, ref = _expect(op, "targets", targets, _IDS, (rows,), device), _expect(op, "ref_logp", ref_logp, _F32, (rows,), device)
@@ -197,13 +198,14 @@ def preference_grad(logits, targets, seq_starts, ref_logp=None, kind="sigmoid", 
         raise SeraphError(f"{op}: kind has to be one of {sorted(PREFERENCE_KINDS)}; got {kind!r}")
     grad = torch.empty_like(logits) if grad is None else grad
     g = _expect(op, "grad", grad, _F32, (rows, cols), device)
+    lp = _expect(op, "logp", logp, _F32, (rows,), device)
     loss = torch.empty(batch // 2, dtype=torch.float32, device=device)
     scores = torch.empty(batch, dtype=torch.float32, device=device)
     k = kernels()
     nbytes = k.seraph_preference_grad_ws_bytes(rows, cols)
     ws = _scratch(nbytes, device)
     options = PreferenceOptions(PREFERENCE_KINDS[kind], beta, label_smoothing, margin, 1 if average else 0)
-    _call(op, device, k.seraph_preference_grad, logits.data_ptr(), t, ref, g, loss.data_ptr(), scores.data_ptr(), None, options, st, batch // 2,
+    _call(op, device, k.seraph_preference_grad, logits.data_ptr(), t, ref, g, loss.data_ptr(), scores.data_ptr(), lp, options, st, batch // 2,
           rows, cols, _ptr(ws), nbytes)
     return grad, loss, scores
 

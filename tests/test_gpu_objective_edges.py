@@ -123,3 +123,36 @@ def test_kl_estimate_far_from_the_reference(ops):
     assert np.abs(logp.cpu().numpy()).max() <= 1e-7
     check("k", kl, want, tol)
     check("loss", loss, 0.5 * want, 0.5 * tol + ref.HALF_STEP * 0.5 * want)
+
+
+@pytest.mark.parametrize("rows,cols", PAIR_FORMS + [(520, 151936)])
+def test_preference_over_the_logits_and_its_log_probabilities(ops, rows, cols):
+    """The gradient written over the logits, as a training step has it, and the optional log-probabilities, in every form; rows ahead of
+    the first sequence, behind the last and in between that are not supervised have 0."""
+    z, t, starts, refl = pair_inputs(rows, cols, cols + 53)
+    starts = starts.copy()
+    starts[0], starts[-1] = 1, rows - 1
+    t[starts[2] + 1] = cols
+    live = ref.supervised(rows, cols, t, None, starts)
+    kw = dict(ref_logp=dev(refl), beta=0.3, label_smoothing=0.1, average=True)
+    S, T = dev(starts.astype(np.uint32)), dev(t)
+    plain = ops.preference_grad(dev(z), T, S, **kw)
+    Z, logp = dev(z), torch.full((rows,), float("nan"), device="cuda")
+    inside = ops.preference_grad(Z, T, S, grad=Z, logp=logp, **kw)
+    assert inside[0] is Z and all(torch.equal(a, b) for a, b in zip(plain, inside))
+    want, tol = ref.token_logprobs(z, np.where(live, t, np.uint32(cols)))
+    check("logp", logp, want["logp"], tol["logp"])
+    if rows * cols < 2e7:
+        compare(dict(zip(("grad", "loss", "scores"), inside)), ref.preference(z, t, starts, ref=refl, beta=0.3, eps=0.1, average=True), f"{rows} x {cols}")
+
+
+def test_refused_log_probabilities(ops):
+    from seraph_amd._lib import SeraphError
+    z, t, s = torch.zeros(4, 8, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"), torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    f = torch.zeros(4, device="cuda")
+    for bad in (f[:3], f.double(), f.cpu(), f.expand(2, 4)[:, 0], z[:, 0]):
+        with pytest.raises(SeraphError, match="logp"):
+            ops.preference_grad(z, t, s, logp=bad)
+    for bad in (dict(logp=f, ref_logp=f), dict(logp=z.view(-1)[4:8])):
+        with pytest.raises(SeraphError, match="overlap"):
+            ops.preference_grad(z, t, s, **bad)
