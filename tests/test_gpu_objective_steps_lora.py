@@ -1,0 +1,96 @@
+"""Steps of a LoRA trainer on the policy and the distillation objective, and the teacher's types and own logsumexp as a step takes
+them, against a float64 autograd statement of model and objective.  Bars as in test_gpu_objective_steps.py."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from tests import refmodel
+from tests.test_gpu_objective_steps import MODEL, STARTS, live_rows, logits_of, next_tokens, policy_loss, setup, tr      # noqa: F401
+from tests.test_gpu_step import check_tensors, rng, tensor_slices
+
+pytestmark = pytest.mark.gpu
+
+LORA = dict(lora_rank=4, lora_alpha=8.0, lora_mask=0b1111111)
+
+
+def f64(a):
+    return torch.from_numpy(np.asarray(a, np.float64))
+
+
+def lora_setup(tr, orc, seed):      # noqa: F811
+    ocfg, p, tok, t = setup(tr, orc, MODEL, seed, **LORA)
+    ad = (0.05 * rng(seed + 1).standard_normal(t.nlora)).astype(np.float32)
+    t.upload(tr.LORA_PARAMS, ad)
+    flat = torch.tensor(ad, dtype=torch.float64, requires_grad=True)
+    P = refmodel.split_params(ocfg, torch.tensor(p, dtype=torch.float64))
+    return ocfg, tok, t, flat, logits_of(ocfg, P, tok, STARTS, refmodel.split_lora(ocfg, flat))
+
+
+def check_step(tr, t, want, flat, loss):      # noqa: F811
+    g, = torch.autograd.grad(want, flat, retain_graph=True)
+    assert abs(loss - want.item()) <= 1e-5 * max(1.0, abs(want.item()))
+    grads = t.download(tr.LORA_GRADS).astype(np.float64)
+    assert np.abs(g.numpy()).max() > 1e-3 and (np.abs(grads - g.numpy()) <= 1e-5 + 1e-4 * np.abs(g.numpy())).all()
+
+
+def own_lse_loss(logits, nxt, live, a, temperature, soft, hard):
+    lp = torch.log_softmax(logits / temperature, 1).gather(1, a["ids"])
+    lq = a["teacher"] / temperature - a["lse"][:, None]
+    kl = (lq.exp() * (lq - lp)).sum(1)
+    label = -torch.log_softmax(logits, 1)[torch.arange(len(nxt)), nxt]
+    return ((soft * kl + hard * label) * a["w"])[live].sum() / live.sum()
+
+
+def test_lora_steps_on_policy_and_distillation(tr, orc):      # noqa: F811
+    ocfg, tok, t, flat, logits = lora_setup(tr, orc, 61)
+    T, V, r = len(tok), MODEL["vocab"], rng(63)
+    w = r.choice([0.0, 0.5, 1.5], T).astype(np.float32)
+    live, nxt = live_rows(T, w), next_tokens(tok)
+    lsm = torch.log_softmax(logits, 1)
+    now = lsm.detach()[torch.arange(T), nxt].numpy()
+    adv, old, ref = r.standard_normal(T).astype(np.float32), (now - 0.07).astype(np.float32), (now + 0.2 * r.standard_normal(T)).astype(np.float32)
+    arrays = dict(adv=f64(adv), old=f64(old), ref=f64(ref), w=f64(w))
+    loss = t.step_policy(tok, STARTS, adv, old, ref_logp=ref, weights=w, clip=(0.2, 0.25), kl_coef=0.05, entropy_coef=0.01, run_optimizer=False)
+    check_step(tr, t, policy_loss(lsm, nxt, live, arrays), flat, loss)
+
+    ids = np.stack([r.permutation(V)[:7] for _ in range(T)]).astype(np.uint32)
+    teacher = (2 * r.standard_normal((T, 7))).astype(np.float32)
+    lse = (np.log(np.exp(teacher / 1.5).sum(1)) + 0.3 * r.random(T)).astype(np.float32)      # the list is most of the distribution
+    arrays.update(ids=torch.from_numpy(ids.astype(np.int64)), lse=f64(lse), teacher=f64(teacher))
+    kw = dict(temperature=1.5, soft_coef=2.0, hard_coef=0.3, weights=w, teacher_lse=lse)
+    loss = t.step_distill(tok, STARTS, ids, teacher, run_optimizer=False, **kw)
+    want = own_lse_loss(logits, nxt, live, arrays, 1.5, 2.0, 0.3)
+    check_step(tr, t, want, flat, loss)
+    before = t.download(tr.LORA_PARAMS)
+    t.step_distill(tok, STARTS, ids, teacher, **kw)
+    assert t.optimizer_step == 1 and (t.download(tr.LORA_PARAMS) != before).any()
+    t.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("top_k", [1, 7, 300])
+def test_the_teachers_types_through_the_step(tr, orc, dtype, top_k):      # noqa: F811
+    """All three types as the C interface takes them, lists longer than the vocabulary among them."""
+    from seraph_amd._lib import DistillOptions
+    from seraph_amd.trainer import _lib
+    ocfg, p, tok, t = setup(tr, orc, MODEL, 71)
+    T, V, r = len(tok), MODEL["vocab"], rng(73)
+    ids = r.integers(0, V, (T, top_k)).astype(np.uint32)
+    teacher = torch.from_numpy((2 * r.standard_normal((T, top_k))).astype(np.float32)).to(dtype)
+    held = teacher.contiguous().view(torch.int32 if dtype == torch.float32 else torch.int16).numpy()
+    flat = torch.tensor(p, dtype=torch.float64, requires_grad=True)
+    logits = logits_of(ocfg, refmodel.split_params(ocfg, flat), tok, STARTS)
+    live = live_rows(T, np.ones(T))
+    arrays = dict(ids=torch.from_numpy(ids.astype(np.int64)), teacher=teacher.double(), w=torch.ones(T, dtype=torch.float64),
+                  lse=torch.logsumexp(teacher.double(), 1))
+    want = own_lse_loss(logits, next_tokens(tok), live, arrays, 1.0, 1.0, 0.0)
+    g, = torch.autograd.grad(want, flat)
+    loss = C.c_float()
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    rc = _lib().hip_train_step_distill(t._h, tok.ctypes.data, T, STARTS.ctypes.data, len(STARTS) - 1, ids.ctypes.data, held.ctypes.data, None, top_k,
+                                       None, DistillOptions(1.0, 1.0, 0.0, code), 0, C.byref(loss))
+    assert rc == 0 and abs(loss.value - want.item()) <= 1e-5 * max(1.0, abs(want.item()))
+    check_tensors(t.download(tr.GRADS), g.numpy(), tensor_slices(ocfg), "grad")
+    t.close()
