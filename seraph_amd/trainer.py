@@ -234,6 +234,8 @@ class Trainer:
                      hard_coef=0.0, run_optimizer=True):
         """A step on distillation from a teacher's listed logits [tokens, top_k] (float32 or float16 arrays)."""
         tp, total, sp, batch, keep = self._batch(tokens, seq_starts)
+        if teacher_ids is None or teacher_logits is None:
+            raise SeraphError("a distillation step needs teacher_ids and teacher_logits")
         teacher_logits = np.asarray(teacher_logits)
         half = teacher_logits.dtype == np.float16
         top_k = teacher_logits.shape[1] if teacher_logits.ndim == 2 else 0
