@@ -704,6 +704,19 @@ static int upload_objective(hip_trainer_t* t, objective_t* o, int T, int batch) 
     return 0;
 }
 
+/* Offsets from 0 to T with one token at least in every sequence (NULL: one sequence). */
+static int check_offsets(const int* seq_starts, int batch, int T) {
+    if (!seq_starts) {
+        if (batch == 1) return 0;
+    } else if (seq_starts[0] == 0 && seq_starts[batch] == T) {
+        for (int b = 0; b < batch; b++)
+            if (seq_starts[b + 1] <= seq_starts[b]) { fprintf(stderr, "ERROR: empty or decreasing sequence %d in seq_starts\n", b); return -1; }
+        return 0;
+    }
+    fprintf(stderr, "ERROR: seq_starts must run from 0 to total_tokens\n");
+    return -1;
+}
+
 static int upload_batch(hip_trainer_t* t, const int* tokens, int T, const int* seq_starts, int batch, const objective_t* obj) {
     uint32_t* tok = t->h_stage;
     uint32_t* tgt = tok + T;
@@ -848,6 +861,8 @@ static float run_step(hip_trainer_t* t, const int* tokens, int total_tokens, con
     const int64_t qd = (int64_t)H * D, kv = (int64_t)KVH * D;
     const float scale = 1.0f / sqrtf((float)D);
     const float eps = c->rms_eps, theta = c->rope_theta > 0 ? c->rope_theta : 10000.0f;
+    /* (ahead of the batches without a prediction, which end here; those of the cross entropy end as the reference's do) */
+    if (obj && check_offsets(seq_starts, batch, total_tokens)) return -1.0f;
     int num_valid = total_tokens - batch;                               /* src/train_cuda.c:1989-1991 */
     if (num_valid <= 0 && !(obj && obj->kind == OBJ_PREFERENCE)) return 0.0f;      /* (a pair has its loss without a prediction too) */
     if (obj && obj->kind != OBJ_LOGPROBS) {                             /* the predictions that count: not the prompts', not a sequence's last */

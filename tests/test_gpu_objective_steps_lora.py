@@ -94,3 +94,22 @@ def test_the_teachers_types_through_the_step(tr, orc, dtype, top_k):      # noqa
     assert rc == 0 and abs(loss.value - want.item()) <= 1e-5 * max(1.0, abs(want.item()))
     check_tensors(t.download(tr.GRADS), g.numpy(), tensor_slices(ocfg), "grad")
     t.close()
+
+
+def test_offsets_that_do_not_fit_are_refused_whatever_counts(tr, orc):      # noqa: F811
+    """Also where no prediction would count: an empty sequence among as many sequences as tokens is no batch without predictions."""
+    from seraph_amd._lib import SeraphError
+    ocfg, p, tok, t = setup(tr, orc, MODEL, 81)
+    T = len(tok)
+    f, ids, z = np.zeros(T, np.float32), np.zeros((T, 2), np.uint32), np.zeros((T, 2), np.float32)
+    short = np.array([0, 1, 1, 2, 4], np.int32)                   # tokens 2 and 3 are one sequence, which has a prediction
+    for starts in (short, np.array([0, 2, 1, 4], np.int32), np.array([0, 1, 2, 3], np.int32), np.array([1, 2, 3, 4], np.int32)):
+        for call in (lambda s: t.token_logprobs(tok[:4], s), lambda s: t.step_policy(tok[:4], s, f[:4], f[:4], weights=f[:4]),
+                     lambda s: t.step_distill(tok[:4], s, ids[:4], z[:4], weights=f[:4])):
+            with pytest.raises(SeraphError):
+                call(starts)
+    with pytest.raises(SeraphError):
+        t.step_preference(tok[:4], short, supervised=f[:4])
+    assert (t.token_logprobs(tok[:4], np.arange(5, dtype=np.int32)) == 0).all()
+    assert (t.download(tr.PARAMS) == p).all() and t.optimizer_step == 0
+    t.close()
