@@ -721,14 +721,13 @@ static int upload_batch(hip_trainer_t* t, const int* tokens, int T, const int* s
     uint32_t* tok = t->h_stage;
     uint32_t* tgt = tok + T;
     uint32_t* st = tgt + T;
+    if (check_offsets(seq_starts, batch, T)) return -1;          /* before anything is written by them */
     for (int b = 0; b <= batch; b++) st[b] = seq_starts ? (uint32_t)seq_starts[b] : (b == 0 ? 0u : (uint32_t)T);
-    if (st[0] != 0 || st[batch] != (uint32_t)T) { fprintf(stderr, "ERROR: seq_starts must run from 0 to total_tokens\n"); return -1; }
     t->attn_pairs = 0.0;
     t->max_seq_len = 1;
     for (int b = 0; b < batch; b++) {
-        if (st[b + 1] > st[b] && (int64_t)(st[b + 1] - st[b]) > t->max_seq_len) t->max_seq_len = st[b + 1] - st[b];
-        if (st[b + 1] > st[b]) t->attn_pairs += 0.5 * (double)(st[b + 1] - st[b]) * (double)(st[b + 1] - st[b] + 1);
-        if (st[b + 1] <= st[b]) { fprintf(stderr, "ERROR: empty or decreasing sequence %d in seq_starts\n", b); return -1; }
+        if ((int64_t)(st[b + 1] - st[b]) > t->max_seq_len) t->max_seq_len = st[b + 1] - st[b];
+        t->attn_pairs += 0.5 * (double)(st[b + 1] - st[b]) * (double)(st[b + 1] - st[b] + 1);
         for (uint32_t i = st[b]; i < st[b + 1]; i++) {                     /* src/train_cuda.c:2029-2043 */
             tok[i] = tokens[i] < 0 ? 0u : (uint32_t)tokens[i];
             tgt[i] = (i + 1 < st[b + 1]) ? (tokens[i + 1] < 0 ? 0u : (uint32_t)tokens[i + 1]) : 0u;

@@ -113,3 +113,20 @@ def test_offsets_that_do_not_fit_are_refused_whatever_counts(tr, orc):      # no
     assert (t.token_logprobs(tok[:4], np.arange(5, dtype=np.int32)) == 0).all()
     assert (t.download(tr.PARAMS) == p).all() and t.optimizer_step == 0
     t.close()
+
+
+def test_offsets_past_the_batch_are_refused_before_use(tr, orc):      # noqa: F811
+    """In the middle of the offsets too, where first and last fit: the host's staging room ends with the batch."""
+    from seraph_amd._lib import SeraphError
+    ocfg, p, tok, t = setup(tr, orc, MODEL, 91)
+    T = len(tok)
+    f = np.ones(T, np.float32)
+    for middle in ([1 << 20], [2, 1 << 30], [1 << 28, 5]):
+        starts = np.array([0] + middle + [T], np.int32)
+        assert t.eval_forward(tok, starts) == -1.0
+        for call in (lambda: t.step(tok, starts), lambda: t.token_logprobs(tok, starts), lambda: t.step_policy(tok, starts, f, f)):
+            with pytest.raises(SeraphError):
+                call()
+    ref_loss, _ = orc.step_full(ocfg, p, tok, STARTS)
+    assert abs(t.step(tok, STARTS, run_optimizer=False) - ref_loss) < 1e-5 * max(1.0, abs(ref_loss))
+    t.close()
