@@ -121,8 +121,9 @@ float hip_evaluate(hip_trainer_t* t, const int* val_tokens, int num_val_tokens, 
  * entries; entry r belongs to the prediction made at token r, whose target is token r + 1 of its sequence (entries of
  * a sequence's last token are ignored).  A prediction whose weight, or whose `supervised` byte, is 0 does not count:
  * mark prompts so.  Policy and distillation losses are the sum over the predictions that count, divided by their number.
- * Return 0 and the loss, which may be negative, in *loss (NAN where the NaN check stopped the step); -1 on error.  A batch
- * without a prediction that counts changes nothing and has the loss 0 (a preference step still steps).
+ * Return 0 and the loss, which may be negative, in *loss (NAN where the NaN check stopped the step); -1 on error, among them
+ * batches of fewer than two tokens and offsets that do not run from 0 to total_tokens with a token at least in each sequence.
+ * A batch without a prediction that counts changes nothing and has the loss 0 (a preference step still steps).
  *
  * hip_token_logprobs is the pass that policy and reference log-probabilities come from: forward only, one value for each
  * prediction (0 for the last token of a sequence), entropy optional.  use_adapters = 0 leaves the adapters of a LoRA

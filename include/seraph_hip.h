@@ -123,11 +123,16 @@ void seraph_cross_entropy_exchange_spins(int spins);
  *
  * A row is supervised when its target is below cols, its weight (where the op has weights) is not 0 and, with
  * seq_starts, it lies in a sequence and is not that sequence's last token.  Any other row is not read: its gradient
- * row and its per-row results are zeros.  Rows behind the last sequence count among those.  Within a supervised row
- * a logit of -inf is an entry that cannot be chosen (probability and gradient 0).
+ * row and its per-row results are zeros.  Rows behind the last sequence count among those.
+ * Within a supervised row a logit of -inf is an entry that cannot be chosen: its probability is 0, and its gradient too unless it is
+ * the row's target or has mass in a teacher's list, where a log-probability of -inf enters the loss.  A row of nothing
+ * but -inf has no distribution: it is NaN, like a row with NaN or +inf in it, and no other row with it (but the rows of its
+ * pair).  exp(logp - old_logp) and exp(ref_logp - logp) are FP32 numbers: where one passes their range (differences
+ * beyond 88), the terms that it enters are not finite.
  * Any cols and any 4-byte aligned buffers are taken.  Results do not depend on the order in which workgroups run.
- * A call without rows or columns does nothing and writes nothing; one holds at most 2^24 - 1 rows (and 2^22 - 1 pairs).  ws needs 16-byte alignment; two calls that may overlap need scratch of
- * their own.  No call allocates, waits or clears by memset, so all of them can be captured into a graph. */
+ * A call without rows or columns does nothing and writes nothing; one holds at most 2^24 - 1 rows (and 2^22 - 1 pairs).
+ * ws needs 16-byte alignment; two calls that may overlap need scratch of their own.  No call allocates, waits or clears by
+ * memset, so all of them can be captured into a graph. */
 
 /* logp[r] = log softmax(logits[r])[targets[r]]; optional (NULL: not wanted) lse[r] = logsumexp of the row and
  * entropy[r] = -sum p log p.  Forward only, for scoring and for the reference / sampling policy's pass. */
@@ -140,7 +145,8 @@ int seraph_token_logprobs(const float* logits, const uint32_t* targets, float* l
  *   loss_rows[r] = w (-min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef k - entropy_coef H),
  *   k = exp(ref_logp - logp) - (ref_logp - logp) - 1   (the non-negative one-sample estimate of KL(policy || reference)),
  * H the entropy of the row, A = advantages[r], w = weights[r] (NULL: 1); grad = d(sum of loss_rows)/d logits / valid_rows.
- * ref_logp is needed where kl_coef != 0 or kl_rows is wanted.  logp_rows, kl_rows, entropy_rows: optional, unweighted. */
+ * ref_logp is needed where kl_coef != 0 or kl_rows is wanted; where it is -inf (a token that the reference masks) k and the loss are
+ * infinite and the gradient is not: k's slope is -1 there.  logp_rows, kl_rows, entropy_rows: optional, unweighted. */
 typedef struct { float clip_low, clip_high, kl_coef, entropy_coef; } seraph_policy_options_t;
 size_t seraph_policy_grad_ws_bytes(int64_t rows, int64_t cols);
 int seraph_policy_grad(const float* logits, const uint32_t* actions, const float* advantages, const float* old_logp,
@@ -156,7 +162,8 @@ int seraph_policy_grad(const float* logits, const uint32_t* actions, const float
  *   HINGE    max(0, 1 - h)
  *   SQUARED  (gap - 1 / (2 beta))^2
  * loss_pairs[pairs], scores[2 pairs] (optional), logp_rows[rows] (optional); grad = d(mean of loss_pairs)/d logits.
- * A sequence without a supervised row has the score 0 and no gradient. */
+ * A sequence without a supervised row has the score 0 and no gradient.  A term of SIGMOID whose factor is 0 is left out, so an
+ * infinite gap has the loss 0 or infinity; a gap that is NaN makes the loss and all of the pair's gradients NaN. */
 #define SERAPH_PREFERENCE_SIGMOID 0
 #define SERAPH_PREFERENCE_HINGE   1
 #define SERAPH_PREFERENCE_SQUARED 2

@@ -17,7 +17,9 @@ namespace seraph {
 
 constexpr int kBlock = 256;
 constexpr int kMaxTopK = 1024;
-constexpr int64_t kMaxRows = 0xffffff;       // a launch holds less than 2^32 lanes, of which a row takes kBlock
+// A launch holds less than 2^32 lanes, of which a row takes 256; those that take 512 (more than 12288 columns) would need more
+// than the card's memory before their rows were too many.
+constexpr int64_t kMaxRows = 0xffffff;
 
 // What a row's list adds up to: the mass sum q and sum q (log q - (z - at) / T), `at` being the largest listed logit of the
 // student (the row's maximum, which the loss needs instead, may not be known yet; differences of logits keep their
@@ -943,9 +945,17 @@ static int streamed_runs(int64_t rows, int64_t cols) {
     const int64_t n = wanted < most ? wanted : most;
     return (int)(n < 1 ? 1 : n > kMaxRuns ? kMaxRuns : n);
 }
-// Few rows, each short enough for one workgroup of 1024 lanes: one launch instead of two.  One CU takes 11.4 us for the
-// exponentials of 151936 columns, which is what the second launch costs (8 rows: 11.4 us against 12.2 us in a sequence of calls);
-// longer rows are better cut.
+// Few rows, each short enough for one workgroup of 1024 lanes: one launch instead of two.  A row's exponentials take one CU about
+// 5.2 us per 100000 columns, on top of the 3 us of any launch; a second launch costs the host 4 us, and little in a
+// captured graph.  Whole / cut, us a call in a sequence of calls (in a graph):
+//              32800 columns           50021                 98304                 151936                163840
+//     1 row    7.4 / 12 (4.9 / 5.4)    7.3 / 12 (6.4 / 5.8)  7.8 / 12 (8.2 / 5.4)  11 / 12 (11 / 5.8)    11 / 12 (11 / 5.3)
+//     8 rows   7.4 / 12 (5.3 / 6.2)    7.4 / 12 (6.8 / 6.4)  8.1 / 12 (8.3 / 5.9)  15 / 12 (14 / 7.0)    13 / 12 (14 / 6.0)
+//    64 rows   7.5 / 12 (6.1 / 7.4)    8.3 / 12 (8.5 / 8.5)  11 / 12 (11 / 9.1)    17 / 13 (17 / 12)     16 / 12 (16 / 11)
+//   128 rows   7.4 / 12 (6.8 / 8.7)    8.8 / 12 (9.0 / 10)   12 / 12 (12 / 13)     18 / 18 (18 / 18)     18 / 17 (18 / 17)
+//   256 rows   8.2 / 12 (8.3 / 12)     11 / 14 (11 / 14)     18 / 19 (18 / 19)     26 / 30 (26 / 29)     28 / 29 (28 / 29)
+// (8 rows of 151936 columns took 11.4 us in other buffers.)  So the limits give away up to 5 us at 8 to 64 rows of 151936 columns and
+// more, and in graphs at few rows beyond 50000.
 static bool in_one_run(int64_t rows, int64_t cols) { return rows <= 256 && cols <= 163840; }
 static size_t streamed_ws_bytes(int64_t rows, int64_t cols) {
     return rows > 0 && cols > 32768 && !in_one_run(rows, cols) ? up16((size_t)rows * streamed_runs(rows, cols) * sizeof(RowStats)) : 0;
@@ -1430,7 +1440,8 @@ int seraph_distill_grad(const float* logits, const uint32_t* teacher_ids, const 
     if (options->soft_coef == 0.0f) top_k = 0;                    // the list is not read: 0 times what it holds need not be 0
     DistillOp op{{nullptr, weights, seq_starts, batch, cols}, {teacher_ids, teacher_logits, teacher_lse, options->teacher_type, (int)top_k},
                  targets, loss_rows, options->soft_coef, options->hard_coef, scale, ExpScale::of(1.0 / (double)options->temperature), 1.0 / (double)options->temperature};
-    // at T = 1 the two parts share their exponentials, at T = 2 one is the other's square
+    // At T = 1 the two parts share their exponentials, at T = 2 one is the other's square; any other T takes two for each logit.  T = 1,
+    // 2 and 1.5: 98.6, 99.4 and 105.4 us at 2047 x 32000 with 256 listed, 867, 872 and 894 us at 4096 x 151936 with 64.
     if (options->hard_coef != 0.0f && options->temperature == 2.0f) return launch_rows<DistillOp, kSquare>(op, logits, grad, rows, cols, top_k, ws, as_stream(s));
     if (options->hard_coef != 0.0f && options->temperature != 1.0f) return launch_rows<DistillOp, kSecond>(op, logits, grad, rows, cols, top_k, ws, as_stream(s));
     return launch_rows<DistillOp, kNone>(op, logits, grad, rows, cols, top_k, ws, as_stream(s));
