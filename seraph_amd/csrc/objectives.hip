@@ -849,21 +849,32 @@ static int launch_shared(const Op& op, const float* logits, float* grad, int64_t
 }
 
 // ---------------------------------------------------------------- long rows read once
-// Forward only: nothing has to be held.  A row is cut into `splits` runs of vectors, each streamed by one workgroup that keeps
-// a running maximum and sums per lane; one wave per row then puts the runs' results together.  Splitting serves
-// few rows, which alone would leave most of the chip idle, and evens out the last round of many.  A row in one run (runs
-// NULL) is finished by its own workgroup.
+// Forward only (T = 1): nothing has to be held.  A row is cut into `splits` runs of vectors, each streamed by one workgroup whose
+// waves keep a running reference value each and sums per lane; one wave per row then puts the runs' results together.
+// Splitting serves few rows, which alone would leave most of the chip idle, and evens out the last round of many.  A row in
+// one run (runs NULL) is finished by its own workgroup.
+//
+// A wave's reference is the maximum of its first batch and stays, as long as no logit exceeds it by kSlack: FP32 sums e^(z - m) as well
+// above 1 as below, and sums that are not rescaled take no second exponential, whose error (exp_below) would be the same for
+// all of the row.  Results of waves and of runs are joined in 64 bits for the same reason.
+constexpr float kSlack = 16.0f;
+
+// The results that the lanes of a wave hold, put together.
 template <int EXTRA>
-__device__ __forceinline__ void add_logit(RowStats& st, float z, ExpScale k) {
-    const float e = exp_of(z, st.m, k);
-    st.s += e;
-    if (EXTRA != kNone) st.x += extra_of<EXTRA>(z, st.m, e);
+__device__ __forceinline__ RowStats join_lanes(RowStats got) {
+    static_assert(EXTRA == kNone || EXTRA == kEntropy, "at T = 1");
+    const float m = wave_top(got.m);
+    const double below = (double)got.m - (double)m, r = exp_below(below);
+    const double s = got.s == 0.0f ? 0.0 : (double)got.s * r;
+    double x = 0.0;
+    if (EXTRA == kEntropy) x = got.s == 0.0f || r == 0.0 ? 0.0 : ((double)got.x + below * (double)got.s) * r;
+    return RowStats{m, (float)wave_total(s), EXTRA != kNone ? (float)wave_total(x) : 0.0f};
 }
 
 template <class Op, int EXTRA, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void streamed_rows_kernel(Op op, const float* logits, int64_t cols, int splits, RowStats* runs) {
     constexpr int kAhead = 8;                                     // vectors in flight per lane
-    __shared__ float red[3][BLOCK / 64];
+    __shared__ RowStats waves[BLOCK / 64];
     const int64_t row = blockIdx.x / (unsigned)splits;
     const int run = (int)(blockIdx.x % (unsigned)splits);
     if (!op.live(row)) {
@@ -878,52 +889,64 @@ __global__ __launch_bounds__(BLOCK) void streamed_rows_kernel(Op op, const float
     const int per_run = ((sh.n4 + splits - 1) / splits + BLOCK - 1) / BLOCK * BLOCK;
     const int first = run * per_run, end = first + per_run < sh.n4 ? first + per_run : sh.n4;
     const ExpScale ks = op.k;
-    RowStats st{kLowest, 0.0f, 0.0f};
-    auto raise = [&](float m) {                                   // a new running maximum
-        if (m > st.m) {
-            st = against<EXTRA>(st, m, ks);
-            st.m = m;
-        }
+    const int lane = (int)threadIdx.x & 63;
+    RowStats st{kLowest, 0.0f, 0.0f};                             // m is the same for the whole wave
+    auto refer_to = [&](float m) {                                // (every lane of the wave is here)
+        if (!__any(m > st.m + kSlack)) return;
+        m = wave_top(fmaxf(m, st.m));
+        st = against<EXTRA>(st, m, ks);
     };
     auto take = [&](const f4 (&v)[kAhead]) {
         float m = kLowest;
 #pragma unroll
         for (int j = 0; j < kAhead; j++) m = fmaxf(m, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
-        raise(m);
+        refer_to(m);
+        float s = 0.0f, ex = 0.0f;                                // a batch's own sums: the lane's take one addition of 32
 #pragma unroll
         for (int j = 0; j < kAhead; j++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) add_logit<EXTRA>(st, v[j][c], ks);
+            for (int c = 0; c < 4; c++) {
+                const float e = exp_of(v[j][c], st.m, ks);
+                s += e;
+                if (EXTRA != kNone) ex += extra_of<EXTRA>(v[j][c], st.m, e);
+            }
+        st.s += s;
+        st.x += ex;
     };
-    int i4 = first + (int)threadIdx.x;
-    for (; i4 + (kAhead - 1) * BLOCK < end; i4 += kAhead * BLOCK) {
+    int base = __builtin_amdgcn_readfirstlane(first + (int)threadIdx.x - lane);      // the wave's first lane's vector
+    for (; base + 63 + (kAhead - 1) * BLOCK < end; base += kAhead * BLOCK) {
         f4 v[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; j++) v[j] = __builtin_nontemporal_load(xv + i4 + j * BLOCK);
+        for (int j = 0; j < kAhead; j++) v[j] = __builtin_nontemporal_load(xv + base + lane + j * BLOCK);
+        __builtin_amdgcn_sched_barrier(0);                        // all loads first: else the scheduler waits for one to save registers
         take(v);
     }
-    if (i4 < end) {                                               // the rest, in flight together as well
+    if (base < end) {                                             // the rest, in flight together as well
         f4 v[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             v[j] = f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (i4 + j * BLOCK < end) v[j] = __builtin_nontemporal_load(xv + i4 + j * BLOCK);
+            if (base + lane + j * BLOCK < end) v[j] = __builtin_nontemporal_load(xv + base + lane + j * BLOCK);
         }
         take(v);
     }
-    const int64_t single = run == 0 ? sh.single((int)threadIdx.x) : -1;
-    if (single >= 0) {
-        const float z = x[single];
-        raise(z);
-        add_logit<EXTRA>(st, z, ks);
+    if (run == 0 && threadIdx.x < 64) {                           // the row's single values
+        const int64_t single = sh.single(lane);
+        const float z = single >= 0 ? x[single] : -INFINITY;
+        refer_to(z);
+        const float e = exp_of(z, st.m, ks);
+        st.s += e;
+        if (EXTRA != kNone) st.x += extra_of<EXTRA>(z, st.m, e);
     }
-    const float m = block_max<BLOCK>(st.m, red[0]);
-    RowStats o = against<EXTRA>(st, m, ks);
-    if (EXTRA != kNone) block_sum2<BLOCK>(o.s, o.x, red[1]);
-    else o.s = block_sum<BLOCK>(o.s, red[1]);
-    if (threadIdx.x == 0) {
-        if (runs) runs[row * splits + run] = RowStats{m, o.s, o.x};
-        else op.template finish<EXTRA>(row, RowStats{m, o.s, o.x}, zt, ListSums{0.0, 0.0, 0.0f});
+    st.s = wave_total(st.s);
+    if (EXTRA != kNone) st.x = wave_total(st.x);
+    if (lane == 0) waves[threadIdx.x >> 6] = st;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    const RowStats o = join_lanes<EXTRA>(lane < BLOCK / 64 ? waves[lane] : RowStats{kLowest, 0.0f, 0.0f});
+    if (lane == 0) {
+        if (runs) runs[row * splits + run] = o;
+        else op.template finish<EXTRA>(row, o, zt, ListSums{0.0, 0.0, 0.0f});
     }
 }
 
@@ -932,10 +955,7 @@ __global__ __launch_bounds__(kBlock) void join_runs_kernel(Op op, const float* l
     const int64_t row = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
     const int lane = (int)threadIdx.x & 63;
     if (row >= rows || !op.live(row)) return;
-    const RowStats got = lane < splits ? runs[row * splits + lane] : RowStats{kLowest, 0.0f, 0.0f};
-    const float m = wave_top(got.m);
-    const RowStats o = against<EXTRA>(got, m, op.k);
-    const RowStats total{m, wave_total(o.s), EXTRA != kNone ? wave_total(o.x) : 0.0f};
+    const RowStats total = join_lanes<EXTRA>(lane < splits ? runs[row * splits + lane] : RowStats{kLowest, 0.0f, 0.0f});
     if (lane == 0) op.template finish<EXTRA>(row, total, logits[row * cols + op.target(row)], ListSums{0.0, 0.0, 0.0f});
 }
 
@@ -1104,10 +1124,11 @@ struct PairRowsOp {
     }
 };
 
-// A row's runs put together, in their order; four loads in flight.
+// A row's runs put together, in their order and in 64 bits (exp_below); four loads in flight.
 __device__ __forceinline__ RowStats joined(const PreferenceArgs& p, int64_t r) {
     const RowStats* runs = p.runs + r * p.splits;
     RowStats st = runs[0];
+    double s = st.s;
     for (int i = 1; i < p.splits; i += 4) {
         RowStats o[4];
 #pragma unroll
@@ -1115,10 +1136,12 @@ __device__ __forceinline__ RowStats joined(const PreferenceArgs& p, int64_t r) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
             if (i + j < p.splits) {
-                const float m = fmaxf(st.m, o[j].m);
-                st = RowStats{m, against<kNone>(st, m, kUnitScale).s + against<kNone>(o[j], m, kUnitScale).s, 0.0f};
+                const double f = exp_below(-fabs((double)o[j].m - (double)st.m));
+                s = o[j].m > st.m ? fma(s, f, (double)o[j].s) : fma((double)o[j].s, f, s);
+                st.m = fmaxf(st.m, o[j].m);
             }
     }
+    st.s = (float)s;
     return st;
 }
 __device__ __forceinline__ RowFactor factor_of(RowStats st, uint32_t target, double f) {
