@@ -159,3 +159,30 @@ def test_a_row_takes_one_exponential_for_each_logit(ops, rows, cols, calls):
     errors = torch.cat(errors)
     assert abs(float(errors.mean())) <= 5e-9 + 3 * ref.HALF_STEP / len(errors) ** 0.5
     assert float(errors.square().mean().sqrt()) <= ref.HALF_STEP
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 13), (40, 8192), (40, 50021), (300, 50021), (40, 151936), (300, 151936), (3, 1300003)])
+@pytest.mark.parametrize("odds", [9.2, 4.6])
+def test_a_token_that_is_nearly_certain(ops, rows, cols, odds):
+    """p = 1 - 1e-4 and 0.99 of one entry, wherever in its row it lies: -logp = log(1 + S) with S the others' share, so a sum whose largest
+    term is exactly 1 is off by what its additions round, 2^-24 at most each beside that 1: those of its lane, of its wave (6) and of
+    the workgroup and the runs (24 at most).  The bar counts them all where they are few, and 94 where a lane has more than 64 in
+    two levels.  Rounding errors of a step of 2^-23 have the standard deviation 2^-23 / sqrt(12) = 0.58 * 2^-24 each, n of them sqrt(n)
+    times that, and from 40 rows that is known to a third (1.4 of it is the bar)."""
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    z = torch.empty(rows, cols, device="cuda").normal_(0, 1, generator=g)
+    t = torch.randint(0, cols, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    t[:4] = torch.tensor([0, cols - 1, cols // 2, 3], device="cuda")[:min(4, rows)]
+    z.scatter_(1, t.long()[:, None], -float("inf"))
+    z.scatter_(1, t.long()[:, None], torch.logsumexp(z.double(), 1)[:, None].float() + odds)
+    want = torch.log_softmax(z.double(), 1).gather(1, t.long()[:, None])[:, 0]
+    assert ((want + float(np.log1p(np.exp(-odds)))).abs() < 1e-5).all()
+    n = min(-(-cols // row_lanes(rows, cols)) + 34, 94)
+    got, _, _ = ops.token_logprobs(z, t)
+    assert ((got.double() - want).abs() <= ref.HALF_STEP * (n + want.abs())).all()
+    rms = 1.4 * 0.58 * n ** 0.5 * ref.HALF_STEP
+    assert float((got.double() - want).square().mean().sqrt()) <= rms
+    if rows % 4 == 0:
+        starts = torch.arange(0, rows + 1, 2, dtype=torch.int32, device="cuda")
+        _, _, scores = ops.preference_grad(z, t, starts)
+        assert float((scores.double() - want[0::2]).square().mean().sqrt()) <= rms
