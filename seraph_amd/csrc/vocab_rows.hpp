@@ -32,7 +32,8 @@ struct RowStats { float m, s, x; };
 
 // The factor log2(e) / T in two parts.  Its FP32 rounding alone (1.3e-8 of it at T = 1) shifts every argument the same way,
 // which the logarithm of a sum keeps: 1.3e-8 times the mean of m - z under the softmax, 7e-8 a token where that is 5.5, and
-// a sequence's score adds its tokens up.  With both parts the errors of such tokens measured 7e-9 in the mean, 9e-8 rms.
+// a sequence's score adds its tokens up.  With both parts the errors of such tokens measured 1e-9 to 5e-9 in the mean, 4e-8 to
+// 9e-8 rms.
 struct ExpScale {
     float hi, lo;
     static ExpScale of(double inv_temp) {
