@@ -130,3 +130,19 @@ def test_offsets_past_the_batch_are_refused_before_use(tr, orc):      # noqa: F8
     ref_loss, _ = orc.step_full(ocfg, p, tok, STARTS)
     assert abs(t.step(tok, STARTS, run_optimizer=False) - ref_loss) < 1e-5 * max(1.0, abs(ref_loss))
     t.close()
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "squared"])
+def test_a_checked_preference_step_stops_at_a_pair_without_a_score(tr, orc, kind):      # noqa: F811
+    """NaN in ref_logp, all logits finite: the check finds it in the logits' gradient and no weight moves."""
+    ocfg, p, tok, t = setup(tr, orc, MODEL, 101)
+    ref = np.full(len(tok), -4.0, np.float32)
+    t.enable_nan_check()
+    t.set_nan_dump_prefix(None)
+    loss, _ = t.step_preference(tok, STARTS, ref_logp=ref, kind=kind, beta=0.3, run_optimizer=False)
+    assert np.isfinite(loss) and not t.nan_detected
+    ref[20] = np.nan                                              # a supervised token of the second pair
+    loss, _ = t.step_preference(tok, STARTS, ref_logp=ref, kind=kind, beta=0.3)
+    assert np.isnan(loss) and t.nan_detected
+    assert (t.download(tr.PARAMS) == p).all()
+    t.close()
